@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_PKG)
@@ -46,32 +47,42 @@ def _nvcc() -> str:
 
 
 def build_cuda_lib(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
-    srcs = [os.path.join(_CSRC, f) for f in ("sk_w2a8.cu", "w2a8_umma.cuh", "ptx_sm100.cuh")]
-    srcs.append(os.path.join(_ROOT, "include", "sk_w2a8.h"))
-    extra = [os.path.join(_CSRC, f) for f in os.listdir(_CSRC) if f.endswith((".cuh", ".cu", ".h"))]
-    if force or _newer(CUDA_LIB, set(srcs + extra)):
-        os.makedirs(LIB_DIR, exist_ok=True)
-        cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + \
-              ["-o", CUDA_LIB, os.path.join(_CSRC, "sk_w2a8.cu")]
-        _run(cmd, verbose)
+    """One object per .cu file (compiled side by side, each only when something it includes is newer), one library."""
+    headers = [os.path.join(_CSRC, f) for f in os.listdir(_CSRC) if f.endswith((".cuh", ".h"))] + \
+              [os.path.join(_ROOT, "include", f) for f in ("sk_w2a8.h", "sk_fp8.h")]
+    units = {"sk_w2a8": [h for h in headers if not os.path.basename(h).startswith(("fp8_", "sk_fp8"))],
+             "sk_fp8": [h for h in headers if not os.path.basename(h).startswith("w2a8_")]}
+    os.makedirs(LIB_DIR, exist_ok=True)
+    objects, jobs = [], []
+    for unit, deps in units.items():
+        src, obj = os.path.join(_CSRC, unit + ".cu"), os.path.join(LIB_DIR, unit + ".o")
+        objects.append(obj)
+        if force or _newer(obj, [src] + deps):
+            jobs.append([_nvcc()] + NVCC_FLAGS[:-1] + (["-Xptxas", "-v"] if ptxas_info else []) + ["-c", "-o", obj, src])
+    with ThreadPoolExecutor() as pool:
+        list(pool.map(lambda cmd: _run(cmd, verbose), jobs))
+    if force or jobs or _newer(CUDA_LIB, objects):
+        _run([_nvcc()] + NVCC_FLAGS + ["-o", CUDA_LIB] + objects, verbose)
     return CUDA_LIB
 
 
 def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
-    src = os.path.join(_CSRC, "torch_ext.cpp")
+    srcs = [os.path.join(_CSRC, f) for f in ("torch_ext.cpp", "torch_fp8.cpp")]
     build_cuda_lib(force=False, verbose=verbose)
-    if force or _newer(TORCH_LIB, [src, os.path.join(_ROOT, "include", "sk_w2a8.h")]):
+    if force or _newer(TORCH_LIB, srcs + [os.path.join(_ROOT, "include", f) for f in ("sk_w2a8.h", "sk_fp8.h")]):
         import torch
         from torch.utils import cpp_extension as ce
         incs = [f"-I{p}" for p in ce.include_paths("cuda")]
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-               "-DTORCH_API_INCLUDE_EXTENSION_H", "-Wno-deprecated-declarations"] + incs + \
-              ["-o", TORCH_LIB, src, f"-L{LIB_DIR}", "-lsk_w2a8", f"-L{tlib}", "-lc10", "-lc10_cuda",
-               "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-L/usr/local/cuda/lib64", "-lcudart",
-               "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]
-        _run(cmd, verbose)
+        cxx = ["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+               "-DTORCH_API_INCLUDE_EXTENSION_H", "-Wno-deprecated-declarations"] + incs
+        objects = [os.path.join(LIB_DIR, os.path.basename(src)[:-4] + ".o") for src in srcs]
+        with ThreadPoolExecutor() as pool:
+            list(pool.map(lambda so: _run(cxx + ["-c", "-o", so[1], so[0]], verbose), zip(srcs, objects)))
+        _run(["g++", "-shared", "-o", TORCH_LIB] + objects +
+             [f"-L{LIB_DIR}", "-lsk_w2a8", f"-L{tlib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+              "-L/usr/local/cuda/lib64", "-lcudart", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"], verbose)
     return TORCH_LIB
 
 

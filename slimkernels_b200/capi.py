@@ -74,6 +74,39 @@ SIGNATURES = {
     "sk_w2a8_version": (_int, []),
 }
 
+# The FP8 products of include/sk_fp8.h (same library)
+SK_SCALE_F32, SK_SCALE_E8M0 = 0, 1
+SK_FLOAT_F16, SK_FLOAT_BF16, SK_FLOAT_F32 = 0, 1, 2
+SK_FP8_OPT_ROW_TILE, SK_FP8_OPT_SPLIT_K, SK_FP8_OPT_WAIT_LIMIT_CYCLES, SK_FP8_OPT_TEST_SKIP_COPY = 1, 2, 3, 4
+
+
+class Fp8Rows(ctypes.Structure):
+    _fields_ = [("q", _vp), ("ld", _i64), ("scale", _vp), ("scale_row", _i64), ("scale_block", _i64)]
+
+
+class Fp8Weight(ctypes.Structure):
+    _fields_ = [("q", _vp), ("ld", _i64), ("scale", _vp), ("experts", _i64), ("N", _i64), ("K", _i64)]
+
+
+_rows, _weight = ctypes.POINTER(Fp8Rows), ctypes.POINTER(Fp8Weight)
+# symbol -> (restype, argtypes); must list every function include/sk_fp8.h declares
+FP8_SIGNATURES = {
+    "sk_fp8_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _rows, _int, _vp]),
+    "sk_fp8_prepare_weight": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _int, _vp]),
+    "sk_fp8_gemm": (_int, [_i64, _rows, _weight, _int, _vp, _i64, _int, _vp]),
+    "sk_fp8_linear_workspace_bytes": (_i64, [_i64, _i64, _int]),
+    "sk_fp8_linear": (_int, [_i64, _vp, _int, _i64, _weight, _int, _vp, _i64, _int, _vp, _i64, _vp]),
+    "sk_fp8_grouped_gemm": (_int, [_i64, _rows, _weight, _int, _vp, _vp, _i64, _int, _vp]),
+    "sk_route_workspace_bytes": (_i64, [_i64, _i64]),
+    "sk_route_tokens": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "sk_group_by_expert": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "sk_fp8_experts_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int]),
+    "sk_fp8_experts": (_int, [_i64, _i64, _vp, _int, _i64, _vp, _vp, _vp, _weight, _weight, _int, _vp, _i64, _int, _vp, _i64, _vp]),
+    "sk_fp8_last_device_status": (_int, [_int, ctypes.POINTER(_int)]),
+    "sk_fp8_query_launch": (_int, [_i64, _i64, _i64, _i64, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int)]),
+    "sk_fp8_set_option": (_int, [_int, _i64]),
+}
+
 _lib = None
 
 
@@ -92,7 +125,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
     if not os.path.exists(path):
         raise ImportError(f"{path} is not built; run `python -m slimkernels_b200._build` (needs nvcc, sm_100a)")
     lib = ctypes.CDLL(path)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **FP8_SIGNATURES}.items():
         fn = getattr(lib, name)          # AttributeError if the symbol is not exported
         fn.restype, fn.argtypes = res, args
     _lib = lib

@@ -1,0 +1,391 @@
+// Row kernels around the FP8 products: the quantiser of activations (in place or into the rows of an expert's group), the weight
+// preparation, the router, and the weighted sum of the experts' results.  All are passes over their data that HBM (large calls) or
+// the launch (small ones) bounds.
+#pragma once
+#include "fp8_common.cuh"
+
+namespace sk {
+
+// Elements of an activation or weight tensor: 0 fp16, 1 bf16, 2 fp32.
+template <int TYPE>
+__device__ __forceinline__ float load_element(const void* p, long long i) {
+  if constexpr (TYPE == 2) return ld_global_f32(static_cast<const float*>(p) + i);
+  unsigned short v;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(static_cast<const uint16_t*>(p) + i) : "memory");
+  if constexpr (TYPE == 1) return __uint_as_float(static_cast<uint32_t>(v) << 16);
+  return __half2float(__ushort_as_half(v));
+}
+__device__ __forceinline__ uint4 ld_global_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+// Eight consecutive elements, 16-byte aligned.
+template <int TYPE>
+__device__ __forceinline__ void load_eight(const void* p, long long i, float (&f)[8]) {
+  if constexpr (TYPE == 2) {
+    const uint4 a = ld_global_v4(static_cast<const float*>(p) + i), b = ld_global_v4(static_cast<const float*>(p) + i + 4);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+  } else {
+    const uint4 a = ld_global_v4(static_cast<const uint16_t*>(p) + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (TYPE == 1) {
+        f[2 * j] = __uint_as_float(w[j] << 16);
+        f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        f[2 * j] = v.x;
+        f[2 * j + 1] = v.y;
+      }
+    }
+  }
+}
+
+// x [M, K] -> codes [M, ld_q] and scales, one per row and block of 128 (the rule is fp8_block_exponent's; a block with a value that
+// is not finite has a NaN scale and NaN codes).  Blocks do not depend on one another: 16 lanes hold one, eight elements each.
+// rows != nullptr: row t is written to the rows rows[t * choices .. t * choices + choices - 1] of the result instead (those >= 0),
+// which orders tokens by expert on the way.
+template <int TYPE, bool E8M0, bool VECTOR>
+__global__ void __launch_bounds__(256)
+fp8_quantize_kernel(const void* x, long long ld_x, long long M, int K, uint8_t* q, long long ld_q, void* scale, long long s_row,
+                    long long s_blk, const int* rows, int choices) {
+  // The next kernel may start only when every CTA of this one has passed the wait: what it then reads early (weights) was complete
+  // before this kernel's inputs were.
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  const int kb = (K + kFp8Block - 1) / kFp8Block;
+  const long long total = M * kb;
+  const int l16 = threadIdx.x & 15;
+  for (long long first = blockIdx.x * 16ll; first < total; first += gridDim.x * 16ll) {   // (whole warps stay together)
+    const long long unit = first + (threadIdx.x >> 4);
+    const bool on = unit < total;
+    const long long m = on ? unit / kb : 0;
+    const int b = on ? static_cast<int>(unit - m * kb) : 0;
+    const int k0 = b * kFp8Block + l16 * 8;
+    float f[8];
+    if (VECTOR && on && k0 + 8 <= K) {
+      load_eight<TYPE>(x, m * ld_x + k0, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = on && k0 + j < K ? load_element<TYPE>(x, m * ld_x + k0 + j) : 0.f;
+    }
+    uint32_t a = 0;                                 // bits of |x|: ordered like the values, infinity and NaN above all
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(f[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (!on) continue;
+    const bool bad = not_finite_bits(a);
+    const int e = bad ? 0 : fp8_block_exponent(a);
+    const float inv = pow2f(-e);
+    uint2 code;
+    code.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
+    code.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
+    if (bad) code = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+    for (int c = 0; c < choices; ++c) {
+      long long r = m;
+      if (rows != nullptr) {
+        r = ld_global_int(rows + m * choices + c);
+        if (r < 0) continue;
+      }
+      uint8_t* dst = q + r * ld_q + k0;
+      if (k0 + 8 <= K) {                            // (ld_q is a multiple of 16)
+        *reinterpret_cast<uint2*>(dst) = code;
+      } else {
+        const uint32_t w[2] = {code.x, code.y};
+        for (int j = 0; j < 8 && k0 + j < K; ++j) dst[j] = static_cast<uint8_t>(w[j >> 2] >> (8 * (j & 3)));
+      }
+      if (l16 == 0) store_scale<E8M0>(scale, r * s_row + b * s_blk, e, bad);
+    }
+  }
+}
+
+// w [rows, K] -> codes and one scale per 128 x 128 block; a CTA takes one block.  blockIdx.y counts matrices of w_rows rows whose
+// blocks start anew.
+template <int TYPE, bool E8M0>
+__global__ void __launch_bounds__(256)
+fp8_prepare_weight_kernel(const void* w, long long ld_w, long long matrix, int N, int K, uint8_t* q, long long ld_q, long long q_matrix,
+                          void* scale) {
+  __shared__ uint32_t red[8];
+  const int kb = (K + kFp8Block - 1) / kFp8Block, nb = (N + kFp8Block - 1) / kFp8Block;
+  const int b = blockIdx.x % kb, r = blockIdx.x / kb;
+  const long long in = blockIdx.y * matrix, out = blockIdx.y * q_matrix;
+  const int col = b * kFp8Block + (threadIdx.x & 31) * 4, row0 = r * kFp8Block + (threadIdx.x >> 5);
+  float f[16][4];
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = row0 + 8 * i, k = col + j;
+      f[i][j] = n < N && k < K ? load_element<TYPE>(w, in + n * ld_w + k) : 0.f;
+      a = max(a, __float_as_uint(f[i][j]) & 0x7fffffffu);
+    }
+  a = __reduce_max_sync(0xffffffffu, a);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, red[i]);
+  const bool bad = not_finite_bits(a);
+  const int e = bad ? 0 : fp8_block_exponent(a);
+  const float inv = pow2f(-e);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int n = row0 + 8 * i;
+    if (n >= N || col >= K) continue;
+    uint32_t code = e4m3x2(f[i][0] * inv, f[i][1] * inv) | (e4m3x2(f[i][2] * inv, f[i][3] * inv) << 16);
+    if (bad) code = 0x7f7f7f7fu;
+    uint8_t* dst = q + out + n * ld_q + col;
+    if (col + 4 <= K && (ld_q & 3) == 0) {
+      *reinterpret_cast<uint32_t*>(dst) = code;
+    } else {
+      for (int j = 0; j < 4 && col + j < K; ++j) dst[j] = static_cast<uint8_t>(code >> (8 * j));
+    }
+  }
+  if (threadIdx.x == 0) store_scale<E8M0>(scale, (static_cast<long long>(blockIdx.y) * nb + r) * kb + b, e, bad);
+}
+
+// out[t, :] = round( sum over j of weights[t, j] * y[rows[t, j], :] ), in the order of j; choices with rows < 0 count nothing.
+template <bool BF16, bool VECTOR>
+__global__ void __launch_bounds__(256)
+fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const float* weights, int choices, int T, int H, uint16_t* out,
+                   long long ld_out) {
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  constexpr int kPer = VECTOR ? 8 : 1;
+  const int per_row = (H + kPer - 1) / kPer;
+  const long long total = static_cast<long long>(T) * per_row;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long t = i / per_row;
+    const int h = static_cast<int>(i - t * per_row) * kPer;
+    float acc[8] = {};
+    for (int j = 0; j < choices; ++j) {
+      const int r = ld_global_int(rows + t * choices + j);
+      if (r < 0) continue;
+      const float w = ld_global_f32(weights + t * choices + j);
+      if constexpr (VECTOR) {
+        float f[8];
+        load_eight<BF16 ? 1 : 0>(y, r * ld_y + h, f);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, f[c], acc[c]);
+      } else {
+        acc[0] = fmaf(w, load_element<BF16 ? 1 : 0>(y, r * ld_y + h), acc[0]);
+      }
+    }
+    uint16_t* dst = out + t * ld_out + h;
+    if constexpr (VECTOR) {
+      uint4 v;
+      v.x = pack_out(acc[0], acc[1], BF16);
+      v.y = pack_out(acc[2], acc[3], BF16);
+      v.z = pack_out(acc[4], acc[5], BF16);
+      v.w = pack_out(acc[6], acc[7], BF16);
+      *reinterpret_cast<uint4*>(dst) = v;
+    } else {
+      *dst = round_out(acc[0], BF16);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- router
+// A CTA takes a run of tokens, a warp a run of those; everything is in the order of the choices t * k + j, so the places are those
+// of a stable sort by expert and the same in every run.
+//   pass 1  (TOPK: the k largest logits of each token and their weights) and how many choices each expert got from this CTA
+//   pass 2  (after pass 1 of all CTAs) the experts' first rows, and the place of each choice
+// With one CTA both are one launch.
+constexpr int kRouteWarps = 16;
+struct RouteParams {
+  const void* logits;                   // [T, ld]
+  long long ld;
+  int T, E, k, renormalize;
+  int* ids;                             // [T, k] written by pass 1, or the caller's
+  float* weights;                       // [T, k]
+  int* rows;                            // [T, k]
+  int* offsets;                         // [E + 1]
+  int* counts;                          // [CTAs][E]
+  int per_cta;                          // tokens
+};
+
+// Bits that order like the logits: larger is larger, NaN above all (as a maximum that propagates it has it).
+__device__ __forceinline__ uint32_t ordered_bits(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);      // (-0 and 0 are one value)
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered_bits(uint32_t o) {
+  if (o == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+// One token: lane holds the logits of experts lane, lane + 32, ...  The choice of round j is the largest value left, the lowest
+// expert among equals.
+template <int TYPE, int PER>
+__device__ __forceinline__ void choose_experts(const RouteParams& p, long long t, int lane) {
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = e < p.E ? ordered_bits(load_element<TYPE>(p.logits, t * p.ld + e)) : 0u;   // (0 is below -infinity's bits)
+  }
+  float top = 0.f, sum = 0.f, mine = 0.f;
+  uint32_t first_bits = 0;
+  if (!p.renormalize) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best = max(best, key[i]);
+    first_bits = __reduce_max_sync(0xffffffffu, best);
+    top = from_ordered_bits(first_bits);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.E) sum += expf(from_ordered_bits(key[i]) - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  for (int j = 0; j < p.k; ++j) {
+    uint32_t best = 0;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+    const uint32_t winner = __reduce_max_sync(0xffffffffu, best);
+    const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i == e) key[i] = 0;
+    if (j == 0) { first_bits = winner; top = from_ordered_bits(winner); }
+    const float w = expf(from_ordered_bits(winner) - top);
+    if (p.renormalize) sum += w;
+    if (lane == j) mine = w;
+    if (lane == 0) p.ids[t * p.k + j] = e;
+  }
+  // a token whose logits are all -infinity has no distribution: its weights are zero
+  if (lane < p.k) p.weights[t * p.k + lane] = first_bits == 0x007fffffu ? 0.f : mine / sum;
+}
+
+template <int TYPE, int PER, bool TOPK>
+__device__ __forceinline__ void route_count(const RouteParams& p, int* hist /* [kRouteWarps][E] */) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kRouteWarps * p.E; i += kRouteWarps * 32) hist[i] = 0;
+  __syncthreads();
+  const long long c0 = static_cast<long long>(blockIdx.x) * p.per_cta, c1 = min(static_cast<long long>(p.T), c0 + p.per_cta);
+  const int per_warp = (p.per_cta + kRouteWarps - 1) / kRouteWarps;
+  const long long t0 = min(c1, c0 + static_cast<long long>(warp) * per_warp), t1 = min(c1, t0 + per_warp);
+  if constexpr (TOPK) {
+    for (long long t = t0; t < t1; ++t) choose_experts<TYPE, PER>(p, t, lane);
+    __syncwarp();
+  }
+  for (long long i = t0 * p.k + lane; i < t1 * p.k; i += 32) {
+    const int e = p.ids[i];
+    if (e >= 0 && e < p.E) atomicAdd(hist + warp * p.E + e, 1);      // (integers: the order does not show)
+  }
+  __syncthreads();
+}
+
+// hist: on entry the warps' counts, on return each warp's next place for every expert.  base: the experts' first places of this CTA.
+__device__ __forceinline__ void route_place(const RouteParams& p, int* hist, const int* base) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) {
+    int at = base[e];
+    for (int w = 0; w < kRouteWarps; ++w) {
+      const int n = hist[w * p.E + e];
+      hist[w * p.E + e] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  const long long c0 = static_cast<long long>(blockIdx.x) * p.per_cta, c1 = min(static_cast<long long>(p.T), c0 + p.per_cta);
+  const int per_warp = (p.per_cta + kRouteWarps - 1) / kRouteWarps;
+  const long long t0 = min(c1, c0 + static_cast<long long>(warp) * per_warp), t1 = min(c1, t0 + per_warp);
+  int* next = hist + warp * p.E;
+  for (long long i0 = t0 * p.k; i0 < t1 * p.k; i0 += 32) {
+    const long long i = i0 + lane;
+    const int e = i < t1 * p.k ? p.ids[i] : -1;
+    const bool on = e >= 0 && e < p.E;
+    const uint32_t same = __match_any_sync(0xffffffffu, on ? e : -1);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    const int at = on ? next[e] + before : -1;
+    __syncwarp();
+    if (on && before == 0) next[e] += __popc(same);
+    __syncwarp();
+    if (i < t1 * p.k) p.rows[i] = at;
+  }
+}
+
+// Exclusive sums over the experts of total[] (in place -> first places), by warp 0; the grand total is stored behind them.
+__device__ __forceinline__ void scan_experts(int* total, int E) {
+  if (threadIdx.x < 32) {
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + static_cast<int>(threadIdx.x);
+      const int n = e < E ? total[e] : 0;
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (static_cast<int>(threadIdx.x) >= o) incl += up;
+      }
+      if (e < E) total[e] = carry + incl - n;
+      carry += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (threadIdx.x == 0) total[E] = carry;
+  }
+  __syncthreads();
+}
+
+// Shared memory: [kRouteWarps][E] counts, [E + 1] totals, [E] first places of this CTA.
+__host__ __device__ constexpr int route_smem_bytes(int E) { return (kRouteWarps * E + 2 * E + 1) * 4; }
+
+template <int TYPE, int PER, bool TOPK, bool ONE_CTA>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+route_count_kernel(const RouteParams p) {
+  extern __shared__ int route_smem[];
+  int* hist = route_smem;
+  int* total = hist + kRouteWarps * p.E;
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  route_count<TYPE, PER, TOPK>(p, hist);
+  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) {
+    int n = 0;
+    for (int w = 0; w < kRouteWarps; ++w) n += hist[w * p.E + e];
+    if constexpr (ONE_CTA) total[e] = n; else p.counts[static_cast<long long>(blockIdx.x) * p.E + e] = n;
+  }
+  if constexpr (ONE_CTA) {
+    __syncthreads();
+    scan_experts(total, p.E);
+    for (int e = threadIdx.x; e <= p.E; e += kRouteWarps * 32) p.offsets[e] = total[e];
+    route_place(p, hist, total);
+  }
+}
+
+__global__ void __launch_bounds__(kRouteWarps * 32)
+route_place_kernel(const RouteParams p) {
+  extern __shared__ int route_smem[];
+  int* hist = route_smem;
+  int* total = hist + kRouteWarps * p.E;
+  int* base = total + p.E + 1;
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  route_count<0, 1, false>(p, hist);                 // this CTA's counts by warp, again
+  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) {
+    int before = 0, all = 0;
+    for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
+      const int n = ld_global_int(p.counts + static_cast<long long>(c) * p.E + e);
+      if (c < static_cast<int>(blockIdx.x)) before += n;
+      all += n;
+    }
+    total[e] = all;
+    base[e] = before;
+  }
+  __syncthreads();
+  scan_experts(total, p.E);
+  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) base[e] += total[e];
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= p.E; e += kRouteWarps * 32) p.offsets[e] = total[e];
+  __syncthreads();
+  route_place(p, hist, base);
+}
+
+}  // namespace sk

@@ -1,0 +1,561 @@
+// Launchers of the FP8 products, the router and the expert layers (C ABI: include/sk_fp8.h).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../../include/sk_fp8.h"
+#include "fp8_common.cuh"
+#include "fp8_narrow.cuh"
+#include "fp8_rows.cuh"
+
+namespace sk {
+
+__device__ int g_fp8_status;            // the first wait that ran into its limit on this device, 0: none
+
+namespace {
+
+std::atomic<int64_t> g_options[5];
+
+int cuda_status(cudaError_t e) {
+  if (e == cudaSuccess) return SK_OK;
+  (void)cudaGetLastError();
+  return e == cudaErrorMemoryAllocation ? SK_ERR_OUT_OF_MEMORY : SK_ERR_CUDA;
+}
+
+struct DeviceInfo {
+  int sms = 0;
+  int* status = nullptr;
+};
+// What a launch needs to know of the current device.
+int device_info(DeviceInfo* out) {
+  constexpr int kMax = 64;
+  static std::atomic<int> sms[kMax];
+  static std::atomic<int*> words[kMax];
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return cuda_status(e);
+  if (dev < 0 || dev >= kMax) return SK_ERR_UNAVAILABLE;
+  if (sms[dev].load() == 0) {
+    // (a first call under stream capture: looking the status word up may load the module, which a capture in global mode refuses)
+    struct Relaxed {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      Relaxed() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+      ~Relaxed() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+    } relaxed;
+    int major = 0, n = 0;
+    if (cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev); e != cudaSuccess) return cuda_status(e);
+    if (major != 10) return SK_ERR_UNSUPPORTED_ARCH;
+    if (cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev); e != cudaSuccess) return cuda_status(e);
+    void* word = nullptr;
+    if (cudaError_t e = cudaGetSymbolAddress(&word, g_fp8_status); e != cudaSuccess) return cuda_status(e);
+    words[dev].store(static_cast<int*>(word));
+    sms[dev].store(n);
+  }
+  out->sms = sms[dev].load();
+  out->status = words[dev].load();
+  return SK_OK;
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// Codes [rows, K] in boxes of 128 bytes x box_rows, 128-byte swizzle, zeros outside.
+int codes_map(const void* q, int64_t rows, int64_t K, int64_t ld, int box_rows, CUtensorMap* out) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return SK_ERR_CUDA;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t unit[2] = {1u, 1u};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(q), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? SK_OK
+             : SK_ERR_CUDA;
+}
+
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+constexpr int64_t kIntMax = 0x7fffffff;
+bool aligned(const void* p, int64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool is_scale_type(int t) { return t == SK_SCALE_F32 || t == SK_SCALE_E8M0; }
+bool is_float_type(int t) { return t >= SK_FLOAT_F16 && t <= SK_FLOAT_F32; }
+bool is_out_type(int t) { return t == SK_OUT_F16 || t == SK_OUT_BF16; }
+int64_t scale_bytes(int scale_type) { return scale_type == SK_SCALE_E8M0 ? 1 : 4; }
+
+struct LaunchConfig {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  LaunchConfig(int64_t grid_x, int64_t grid_y, int threads, int64_t smem, bool dependent, int cluster, cudaStream_t stream) {
+    cfg.gridDim = dim3(static_cast<unsigned>(grid_x), static_cast<unsigned>(grid_y), 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 0;
+    if (dependent) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attr[cfg.numAttrs].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+      ++cfg.numAttrs;
+    }
+  }
+};
+
+// Calls fn(std::integral_constant...) for a runtime value.
+template <class F>
+int with_bool(bool b, F&& fn) {
+  return b ? fn(std::true_type{}) : fn(std::false_type{});
+}
+template <class F>
+int with_type(int t, F&& fn) {
+  switch (t) {
+    case 0: return fn(std::integral_constant<int, 0>{});
+    case 1: return fn(std::integral_constant<int, 1>{});
+    default: return fn(std::integral_constant<int, 2>{});
+  }
+}
+
+// ---------------------------------------------------------------- products
+struct Choice {
+  int row_tile, feature_tile, split;
+  int64_t ctas;
+};
+
+// One product, or the products of a group: what decides how it is launched.
+Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, int sms) {
+  Choice c;
+  const int64_t rows = ceil_div(M, experts);       // of a group, on average
+  c.feature_tile = 128;
+  c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || silu ? 64 : 128;
+  if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(silu && forced > 64 ? 64 : forced);
+  const int64_t n_tiles = ceil_div(N, c.feature_tile);
+  const int64_t tiles = (grouped ? ceil_div(M, c.row_tile) + std::min(experts, M) : ceil_div(M, c.row_tile)) * n_tiles;
+  c.split = 1;
+  if (!grouped) {
+    const int64_t kb = ceil_div(K, 128);
+    while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * 4) c.split *= 2;
+    if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
+  }
+  c.ctas = tiles * c.split;
+  return c;
+}
+
+template <int TOK, bool E8M0, bool SILU>
+int launch_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+  using T = Fp8NarrowTraits<TOK, SILU>;
+  auto kern = fp8_narrow_kernel<TOK, E8M0, SILU>;
+  const int smem = T::dynamic_bytes(p.split, p.experts);
+  constexpr int kMost = T::dynamic_bytes(SILU ? 1 : 8, kFp8MaxExperts);
+  static_assert(T::dynamic_bytes(SILU ? 1 : 8, 1) <= 232448 && T::dynamic_bytes(1, kFp8MaxExperts) <= 232448, "shared memory of a CTA");
+  // (an attribute of the function on each device; setting it again costs nothing to speak of)
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, std::min(kMost, 232448)); e != cudaSuccess)
+    return cuda_status(e);
+  const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * T::kCtas);
+  LaunchConfig lc(grid, 1, T::kThreads, smem, dependent, p.split, stream);
+  return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
+}
+
+template <bool E8M0, bool SILU>
+int launch_product(const Choice& c, const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev,
+                   bool dependent, cudaStream_t stream) {
+  switch (c.row_tile) {
+    case 16: return launch_narrow<16, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+    case 32: return launch_narrow<32, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+    case 64: return launch_narrow<64, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+    default:
+      if constexpr (SILU) return SK_ERR_UNAVAILABLE;
+      else return launch_narrow<128, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+  }
+}
+
+// silu_out: the SiLU epilogue; w then holds 2 * experts matrices of N rows.  `dependent`: the previous kernel in the stream is this
+// library's and lets this one start early; early_weights: ... and no kernel that may still run wrote the weights.
+int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_type, const int32_t* offsets, void* out, int64_t ld_out,
+            int out_dtype, const sk_fp8_rows* silu_out, bool dependent, bool early_weights, cudaStream_t stream) {
+  const bool silu = silu_out != nullptr;
+  const int64_t experts = silu ? w->experts / 2 : w->experts;
+  const int64_t N = w->N, K = w->K;
+  DeviceInfo dev;
+  if (int rc = device_info(&dev); rc != SK_OK) return rc;
+  const Choice c = choose(M, N, K, experts, offsets != nullptr, silu, dev.sms);
+  Fp8Params p = {};
+  p.x_scale = x->scale;
+  p.xs_row = x->scale_row;
+  p.xs_blk = x->scale_block;
+  p.w_scale = w->scale;
+  const int64_t blocks = ceil_div(N, 128);
+  p.scale_rows = silu ? 2 * blocks : blocks;
+  p.offsets = offsets;
+  p.experts = offsets ? static_cast<int>(experts) : 1;
+  p.w_rows = static_cast<int>(silu ? 2 * N : N);
+  p.out = silu ? silu_out->q : out;
+  p.ld_out = silu ? silu_out->ld : ld_out;
+  if (silu) {
+    p.h_scale = silu_out->scale;
+    p.hs_row = silu_out->scale_row;
+    p.hs_blk = silu_out->scale_block;
+    p.up_row0 = static_cast<int>(N);
+    p.up_block0 = static_cast<int>(blocks);
+  }
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.k_blocks = static_cast<int>(ceil_div(K, 128));
+  p.n_tiles = static_cast<int>(ceil_div(N, c.feature_tile));
+  p.out_bf16 = out_dtype == SK_OUT_BF16;
+  p.vector_out = !silu && aligned(out, 16) && ld_out % 8 == 0;
+  p.early_weights = early_weights && offsets == nullptr;
+  p.split = c.split;
+  p.skip_block = static_cast<int>(g_options[SK_FP8_OPT_TEST_SKIP_COPY].load()) - 1;
+  const int64_t limit = g_options[SK_FP8_OPT_WAIT_LIMIT_CYCLES].load();
+  p.wait_limit = limit > 0 ? limit : kWaitLimitCycles;
+  p.status = dev.status;
+  const int64_t tiles = c.ctas / c.split;
+  if (tiles > kIntMax / 8) return SK_ERR_BAD_SHAPE;
+  CUtensorMap mw, mx;
+  if (int rc = codes_map(w->q, w->experts * N, K, w->ld, 128, &mw); rc != SK_OK) return rc;
+  if (int rc = codes_map(x->q, M, K, x->ld, c.row_tile, &mx); rc != SK_OK) return rc;
+  return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
+    return with_bool(silu, [&](auto s) {
+      return launch_product<decltype(e8m0)::value, decltype(s)::value>(c, mw, mx, p, tiles, dev, dependent, stream);
+    });
+  });
+}
+
+int check_weight(const sk_fp8_weight* w, int64_t max_experts) {
+  if (!w || !w->q || !w->scale) return SK_ERR_NULL_POINTER;
+  if (w->experts < 1 || w->experts > max_experts || w->N < 1 || w->K < 1 || w->ld < w->K) return SK_ERR_BAD_SHAPE;
+  if (w->N > kIntMax / 256 || w->K > kIntMax / 256 || w->experts * w->N > kIntMax - 4096 || w->ld >= (int64_t(1) << 36)) return SK_ERR_BAD_SHAPE;
+  if (!aligned(w->q, 16) || w->ld % 16) return SK_ERR_BAD_ALIGNMENT;
+  return SK_OK;
+}
+int check_rows(const sk_fp8_rows* x, int64_t M, int64_t K) {
+  if (!x || !x->q || !x->scale) return SK_ERR_NULL_POINTER;
+  if (M < 0 || M > kIntMax - 4096 || x->ld < K || x->ld >= (int64_t(1) << 36)) return SK_ERR_BAD_SHAPE;
+  if (!aligned(x->q, 16) || x->ld % 16) return SK_ERR_BAD_ALIGNMENT;
+  return SK_OK;
+}
+
+int quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t K, const sk_fp8_rows& out, int scale_type, const int32_t* rows,
+             int64_t choices, bool dependent, cudaStream_t stream) {
+  DeviceInfo dev;
+  if (int rc = device_info(&dev); rc != SK_OK) return rc;
+  const int64_t units = M * ceil_div(K, 128);
+  const int64_t grid = std::min<int64_t>(ceil_div(units, 16), static_cast<int64_t>(dev.sms) * 8);
+  const int64_t size = x_type == SK_FLOAT_F32 ? 4 : 2;
+  const bool vector = aligned(x, 16) && ld_x * size % 16 == 0;
+  LaunchConfig lc(grid, 1, 256, 0, dependent, 1, stream);
+  return with_type(x_type, [&](auto type) {
+    return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
+      return with_bool(vector, [&](auto v) {
+        return cuda_status(cudaLaunchKernelEx(&lc.cfg, fp8_quantize_kernel<decltype(type)::value, decltype(e8m0)::value, decltype(v)::value>, x,
+                                              static_cast<long long>(ld_x), static_cast<long long>(M), static_cast<int>(K), out.q,
+                                              static_cast<long long>(out.ld), out.scale, static_cast<long long>(out.scale_row),
+                                              static_cast<long long>(out.scale_block), static_cast<const int*>(rows), static_cast<int>(choices)));
+      });
+    });
+  });
+}
+
+// Codes and scales of [M, K] in a workspace.  8-bit scales lie row by row, 32-bit ones block by block: that is how the
+// products read them, a row's four blocks at once or 32 rows of a block at once.
+int64_t rows_bytes(int64_t M, int64_t K, int scale_type) {
+  return round_up(M * round_up(K, 16), 256) + round_up(M * ceil_div(K, 128) * scale_bytes(scale_type), 256);
+}
+sk_fp8_rows rows_in(uint8_t* at, int64_t M, int64_t K, int scale_type) {
+  const int64_t kb = ceil_div(K, 128), ld = round_up(K, 16);
+  sk_fp8_rows r;
+  r.q = at;
+  r.ld = ld;
+  r.scale = at + round_up(M * ld, 256);
+  r.scale_row = scale_type == SK_SCALE_E8M0 ? kb : 1;
+  r.scale_block = scale_type == SK_SCALE_E8M0 ? 1 : M;
+  return r;
+}
+
+// ---------------------------------------------------------------- router
+// Tokens per CTA: one CTA for as long as its warps have a token or two each, then enough for one CTA per SM.
+int64_t route_per_cta(int64_t T, int sms) {
+  if (T <= 4 * kRouteWarps) return std::max<int64_t>(T, 1);
+  return std::max<int64_t>(2 * kRouteWarps, round_up(ceil_div(T, sms), kRouteWarps));
+}
+
+template <int TYPE, bool TOPK>
+int launch_route(RouteParams p, int64_t ctas, bool dependent, cudaStream_t stream) {
+  const int smem = route_smem_bytes(p.E);
+  const auto go = [&](auto per) -> int {
+    constexpr int kPer = decltype(per)::value;
+    auto one = route_count_kernel<TYPE, kPer, TOPK, true>;
+    auto many = route_count_kernel<TYPE, kPer, TOPK, false>;
+    auto kern = ctas == 1 ? one : many;
+    if (smem > 48 * 1024)
+      if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_status(e);
+    LaunchConfig lc(ctas, 1, kRouteWarps * 32, smem, dependent, 1, stream);
+    if (cudaError_t e = cudaLaunchKernelEx(&lc.cfg, kern, p); e != cudaSuccess) return cuda_status(e);
+    if (ctas == 1) return SK_OK;
+    if (smem > 48 * 1024)
+      if (cudaError_t e = cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess)
+        return cuda_status(e);
+    LaunchConfig second(ctas, 1, kRouteWarps * 32, smem, true, 1, stream);
+    return cuda_status(cudaLaunchKernelEx(&second.cfg, route_place_kernel, p));
+  };
+  if constexpr (!TOPK) {
+    return go(std::integral_constant<int, 1>{});
+  } else {
+    const int per = static_cast<int>(ceil_div(p.E, 32));
+    if (per <= 1) return go(std::integral_constant<int, 1>{});
+    if (per <= 2) return go(std::integral_constant<int, 2>{});
+    if (per <= 4) return go(std::integral_constant<int, 4>{});
+    if (per <= 8) return go(std::integral_constant<int, 8>{});
+    if (per <= 16) return go(std::integral_constant<int, 16>{});
+    return go(std::integral_constant<int, 32>{});
+  }
+}
+
+int route(RouteParams p, int logits_type, bool topk, int64_t T, int64_t E, int64_t k, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  DeviceInfo dev;
+  if (int rc = device_info(&dev); rc != SK_OK) return rc;
+  p.T = static_cast<int>(T);
+  p.E = static_cast<int>(E);
+  p.k = static_cast<int>(k);
+  p.per_cta = static_cast<int>(route_per_cta(T, dev.sms));
+  const int64_t ctas = std::max<int64_t>(1, ceil_div(T, p.per_cta));
+  if (ctas > 1) {
+    if (!workspace) return SK_ERR_NULL_POINTER;
+    if (workspace_bytes < ctas * E * 4) return SK_ERR_BAD_ARGUMENT;
+    if (!aligned(workspace, 4)) return SK_ERR_BAD_ALIGNMENT;
+    p.counts = static_cast<int*>(workspace);
+  }
+  if (!topk) return launch_route<0, false>(p, ctas, false, stream);
+  return with_type(logits_type, [&](auto type) { return launch_route<decltype(type)::value, true>(p, ctas, false, stream); });
+}
+
+int check_route(int64_t T, int64_t E, int64_t k) {
+  if (E < 1 || E > kFp8MaxExperts || k < 1 || k > std::min<int64_t>(E, 32) || T < 0 || T > kIntMax / 64) return SK_ERR_BAD_SHAPE;
+  return SK_OK;
+}
+
+}  // namespace
+}  // namespace sk
+
+using namespace sk;
+
+extern "C" {
+
+int sk_fp8_quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t K, const sk_fp8_rows* out, int scale_type, sk_stream_t stream) {
+  if (!x || !out) return SK_ERR_NULL_POINTER;
+  if (!is_float_type(x_type) || !is_scale_type(scale_type)) return SK_ERR_BAD_ARGUMENT;
+  if (K < 1 || K > kIntMax / 256 || ld_x < K) return SK_ERR_BAD_SHAPE;
+  if (int rc = check_rows(out, M, K); rc != SK_OK) return rc;
+  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2)) return SK_ERR_BAD_ALIGNMENT;
+  if (M == 0) return SK_OK;
+  return quantize(x, x_type, ld_x, M, K, *out, scale_type, nullptr, 1, false, static_cast<cudaStream_t>(stream));
+}
+
+int sk_fp8_prepare_weight(const void* w, int w_type, int64_t ld_w, int64_t w_matrix, int64_t matrices, int64_t N, int64_t K, uint8_t* w_q,
+                          int64_t ld_q, int64_t q_matrix, void* w_scale, int scale_type, sk_stream_t stream) {
+  if (!w || !w_q || !w_scale) return SK_ERR_NULL_POINTER;
+  if (!is_float_type(w_type) || !is_scale_type(scale_type)) return SK_ERR_BAD_ARGUMENT;
+  if (N < 1 || K < 1 || N > kIntMax / 256 || K > kIntMax / 256 || matrices < 1 || matrices > 65535 || ld_w < K || ld_q < K) return SK_ERR_BAD_SHAPE;
+  const int64_t blocks = ceil_div(N, 128) * ceil_div(K, 128);
+  if (blocks > kIntMax) return SK_ERR_BAD_SHAPE;
+  if (!aligned(w, w_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(w_q, 16) || ld_q % 16 || q_matrix % 4) return SK_ERR_BAD_ALIGNMENT;
+  DeviceInfo dev;
+  if (int rc = device_info(&dev); rc != SK_OK) return rc;
+  LaunchConfig lc(blocks, matrices, 256, 0, false, 1, static_cast<cudaStream_t>(stream));
+  return with_type(w_type, [&](auto type) {
+    return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
+      return cuda_status(cudaLaunchKernelEx(&lc.cfg, fp8_prepare_weight_kernel<decltype(type)::value, decltype(e8m0)::value>, w,
+                                            static_cast<long long>(ld_w), static_cast<long long>(w_matrix), static_cast<int>(N), static_cast<int>(K),
+                                            w_q, static_cast<long long>(ld_q), static_cast<long long>(q_matrix), w_scale));
+    });
+  });
+}
+
+static int check_product(int64_t M, const sk_fp8_weight* w, int scale_type, const void* out, int64_t ld_out, int out_dtype, int64_t max_experts) {
+  if (int rc = check_weight(w, max_experts); rc != SK_OK) return rc;
+  if (!out) return SK_ERR_NULL_POINTER;
+  if (!is_scale_type(scale_type) || !is_out_type(out_dtype)) return SK_ERR_BAD_ARGUMENT;
+  if (scale_type == SK_SCALE_F32 && !aligned(w->scale, 4)) return SK_ERR_BAD_ALIGNMENT;
+  if (M < 0 || M > kIntMax - 4096 || ld_out < w->N) return SK_ERR_BAD_SHAPE;
+  if (!aligned(out, 2)) return SK_ERR_BAD_ALIGNMENT;
+  return SK_OK;
+}
+
+int sk_fp8_gemm(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_type, void* out, int64_t ld_out, int out_dtype, sk_stream_t stream) {
+  if (int rc = check_product(M, w, scale_type, out, ld_out, out_dtype, 1); rc != SK_OK) return rc;
+  if (int rc = check_rows(x, M, w->K); rc != SK_OK) return rc;
+  if (scale_type == SK_SCALE_F32 && !aligned(x->scale, 4)) return SK_ERR_BAD_ALIGNMENT;
+  if (M == 0) return SK_OK;
+  return product(M, x, w, scale_type, nullptr, out, ld_out, out_dtype, nullptr, false, false, static_cast<cudaStream_t>(stream));
+}
+
+int sk_fp8_grouped_gemm(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_type, const int32_t* offsets, void* out, int64_t ld_out,
+                        int out_dtype, sk_stream_t stream) {
+  if (int rc = check_product(M, w, scale_type, out, ld_out, out_dtype, kFp8MaxExperts); rc != SK_OK) return rc;
+  if (int rc = check_rows(x, M, w->K); rc != SK_OK) return rc;
+  if (!offsets) return SK_ERR_NULL_POINTER;
+  if (!aligned(offsets, 4) || (scale_type == SK_SCALE_F32 && !aligned(x->scale, 4))) return SK_ERR_BAD_ALIGNMENT;
+  if (M == 0) return SK_OK;
+  return product(M, x, w, scale_type, offsets, out, ld_out, out_dtype, nullptr, false, false, static_cast<cudaStream_t>(stream));
+}
+
+int64_t sk_fp8_linear_workspace_bytes(int64_t M, int64_t K, int scale_type) {
+  if (M < 0 || K < 1 || !is_scale_type(scale_type)) return 0;
+  return rows_bytes(M, K, scale_type);
+}
+
+int sk_fp8_linear(int64_t M, const void* x, int x_type, int64_t ld_x, const sk_fp8_weight* w, int scale_type, void* out, int64_t ld_out, int out_dtype,
+                  void* workspace, int64_t workspace_bytes, sk_stream_t stream) {
+  if (int rc = check_product(M, w, scale_type, out, ld_out, out_dtype, 1); rc != SK_OK) return rc;
+  if (!x || !workspace) return SK_ERR_NULL_POINTER;
+  if (!is_float_type(x_type) || workspace_bytes < rows_bytes(M, w->K, scale_type)) return SK_ERR_BAD_ARGUMENT;
+  if (ld_x < w->K) return SK_ERR_BAD_SHAPE;
+  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(workspace, 256)) return SK_ERR_BAD_ALIGNMENT;
+  if (M == 0) return SK_OK;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const sk_fp8_rows rows = rows_in(static_cast<uint8_t*>(workspace), M, w->K, scale_type);
+  if (int rc = quantize(x, x_type, ld_x, M, w->K, rows, scale_type, nullptr, 1, true, s); rc != SK_OK) return rc;
+  return product(M, &rows, w, scale_type, nullptr, out, ld_out, out_dtype, nullptr, true, true, s);
+}
+
+int64_t sk_route_workspace_bytes(int64_t T, int64_t E) {
+  if (check_route(T, E, 1) != SK_OK) return 0;
+  // (never more CTAs than this, whatever the device)
+  return std::min<int64_t>(ceil_div(std::max<int64_t>(T, 1), 2 * kRouteWarps), 1024) * E * 4;
+}
+
+int sk_route_tokens(const void* logits, int logits_type, int64_t ld, int64_t T, int64_t E, int64_t k, int renormalize, int32_t* ids, float* weights,
+                    int32_t* rows, int32_t* offsets, void* workspace, int64_t workspace_bytes, sk_stream_t stream) {
+  if (!logits || !ids || !weights || !rows || !offsets) return SK_ERR_NULL_POINTER;
+  if (!is_float_type(logits_type)) return SK_ERR_BAD_ARGUMENT;
+  if (int rc = check_route(T, E, k); rc != SK_OK) return rc;
+  if (ld < E) return SK_ERR_BAD_SHAPE;
+  RouteParams p = {};
+  p.logits = logits;
+  p.ld = ld;
+  p.renormalize = renormalize != 0;
+  p.ids = ids;
+  p.weights = weights;
+  p.rows = rows;
+  p.offsets = offsets;
+  return route(p, logits_type, true, T, E, k, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int32_t* rows, int32_t* offsets, void* workspace, int64_t workspace_bytes,
+                       sk_stream_t stream) {
+  if (!ids || !rows || !offsets) return SK_ERR_NULL_POINTER;
+  if (int rc = check_route(T, E, 1); rc != SK_OK) return rc;
+  if (k < 1 || k > 1024) return SK_ERR_BAD_SHAPE;
+  RouteParams p = {};
+  p.ids = const_cast<int32_t*>(ids);               // (only read)
+  p.rows = rows;
+  p.offsets = offsets;
+  return route(p, SK_FLOAT_F32, false, T, E, k, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int64_t sk_fp8_experts_workspace_bytes(int64_t T, int64_t k, int64_t hidden, int64_t inter, int scale_type) {
+  if (T < 0 || k < 1 || hidden < 1 || inter < 1 || !is_scale_type(scale_type)) return 0;
+  return rows_bytes(T * k, hidden, scale_type) + rows_bytes(T * k, inter, scale_type) + round_up(T * k * round_up(hidden, 8) * 2, 256);
+}
+
+int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x, const int32_t* rows, const float* weights, const int32_t* offsets,
+                   const sk_fp8_weight* gate_up, const sk_fp8_weight* down, int scale_type, void* out, int64_t ld_out, int out_dtype, void* workspace,
+                   int64_t workspace_bytes, sk_stream_t stream) {
+  if (!x || !rows || !weights || !offsets || !workspace) return SK_ERR_NULL_POINTER;
+  if (int rc = check_product(T, down, scale_type, out, ld_out, out_dtype, kFp8MaxExperts); rc != SK_OK) return rc;
+  if (int rc = check_weight(gate_up, 2 * kFp8MaxExperts); rc != SK_OK) return rc;
+  if (scale_type == SK_SCALE_F32 && !aligned(gate_up->scale, 4)) return SK_ERR_BAD_ALIGNMENT;
+  const int64_t hidden = down->N, inter = down->K, E = down->experts;
+  if (gate_up->experts != 2 * E || gate_up->N != inter || gate_up->K != hidden || ld_x < hidden) return SK_ERR_BAD_SHAPE;
+  if (k < 1 || k > 1024 || T * k > kIntMax - 4096) return SK_ERR_BAD_SHAPE;
+  if (!is_float_type(x_type) || workspace_bytes < sk_fp8_experts_workspace_bytes(T, k, hidden, inter, scale_type)) return SK_ERR_BAD_ARGUMENT;
+  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(workspace, 256)) return SK_ERR_BAD_ALIGNMENT;
+  if (T == 0) return SK_OK;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t R = T * k, ld_y = round_up(hidden, 8);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  const sk_fp8_rows xr = rows_in(at, R, hidden, scale_type);
+  at += rows_bytes(R, hidden, scale_type);
+  const sk_fp8_rows hr = rows_in(at, R, inter, scale_type);
+  at += rows_bytes(R, inter, scale_type);
+  if (int rc = quantize(x, x_type, ld_x, T, hidden, xr, scale_type, rows, k, true, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &xr, gate_up, scale_type, offsets, nullptr, 0, out_dtype, &hr, true, false, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, out_dtype, nullptr, true, false, s); rc != SK_OK) return rc;
+  DeviceInfo dev;
+  if (int rc = device_info(&dev); rc != SK_OK) return rc;
+  const bool vector = hidden % 8 == 0 && ld_out % 8 == 0 && aligned(out, 16);
+  const int64_t units = T * (vector ? hidden / 8 : hidden);
+  LaunchConfig lc(std::min<int64_t>(ceil_div(units, 256), static_cast<int64_t>(dev.sms) * 8), 1, 256, 0, true, 1, s);
+  return with_bool(out_dtype == SK_OUT_BF16, [&](auto bf16) {
+    return with_bool(vector, [&](auto v) {
+      return cuda_status(cudaLaunchKernelEx(&lc.cfg, fp8_combine_kernel<decltype(bf16)::value, decltype(v)::value>,
+                                            reinterpret_cast<const uint16_t*>(at), static_cast<long long>(ld_y), static_cast<const int*>(rows), weights,
+                                            static_cast<int>(k), static_cast<int>(T), static_cast<int>(hidden), static_cast<uint16_t*>(out),
+                                            static_cast<long long>(ld_out)));
+    });
+  });
+}
+
+int sk_fp8_last_device_status(int device, int* device_status) {
+  if (device_status) *device_status = 0;
+  int cur = 0;
+  if (cudaError_t e = cudaGetDevice(&cur); e != cudaSuccess) return cuda_status(e);
+  if (cudaError_t e = cudaSetDevice(device); e != cudaSuccess) return cuda_status(e);
+  int word = 0;
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&word, g_fp8_status, sizeof(int));
+  if (e == cudaSuccess && word != 0) e = cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int));
+  (void)cudaSetDevice(cur);
+  if (e != cudaSuccess) return cuda_status(e);
+  if (device_status) *device_status = word;
+  return word == 0 ? SK_OK : SK_ERR_DEVICE_TIMEOUT;
+}
+
+int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int* row_tile, int* feature_tile, int* split, int* ctas) {
+  if (M < 1 || N < 1 || K < 1 || experts < 1 || experts > kFp8MaxExperts) return SK_ERR_BAD_SHAPE;
+  DeviceInfo dev;
+  if (int rc = device_info(&dev); rc != SK_OK) return rc;
+  const Choice c = choose(M, N, K, experts, experts > 1, false, dev.sms);
+  if (row_tile) *row_tile = c.row_tile;
+  if (feature_tile) *feature_tile = c.feature_tile;
+  if (split) *split = c.split;
+  if (ctas) *ctas = static_cast<int>(std::min<int64_t>(c.ctas, kIntMax));
+  return SK_OK;
+}
+
+int sk_fp8_set_option(int key, int64_t value) {
+  if (value < 0) return SK_ERR_BAD_ARGUMENT;
+  switch (key) {
+    case SK_FP8_OPT_ROW_TILE:
+      if (value != 0 && value != 16 && value != 32 && value != 64 && value != 128) return SK_ERR_BAD_ARGUMENT;
+      break;
+    case SK_FP8_OPT_SPLIT_K:
+      if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return SK_ERR_BAD_ARGUMENT;
+      break;
+    case SK_FP8_OPT_WAIT_LIMIT_CYCLES:
+      if (value != 0 && value < 1000) return SK_ERR_BAD_ARGUMENT;
+      break;
+    case SK_FP8_OPT_TEST_SKIP_COPY:
+      if (value > kIntMax) return SK_ERR_BAD_ARGUMENT;
+      break;
+    default: return SK_ERR_BAD_ARGUMENT;
+  }
+  g_options[key].store(value);
+  return SK_OK;
+}
+
+}  // extern "C"
