@@ -97,7 +97,7 @@ int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int* r
 
 /* Testing and tuning, process-wide; 0 restores the default. */
 typedef enum sk_fp8_option {
-  SK_FP8_OPT_ROW_TILE = 1,          /* rows per tile */
+  SK_FP8_OPT_ROW_TILE = 1,          /* 16 / 32 / 64 / 128: rows per tile of the kernel for few rows; 256: the kernel for many rows */
   SK_FP8_OPT_SPLIT_K = 2,           /* CTAs that share the K range of a tile (products of one group) */
   SK_FP8_OPT_WAIT_LIMIT_CYCLES = 3, /* as SK_OPT_WAIT_LIMIT_CYCLES */
   SK_FP8_OPT_TEST_SKIP_COPY = 4     /* as SK_OPT_TEST_SKIP_COPY */

@@ -9,6 +9,7 @@
 #include "fp8_common.cuh"
 #include "fp8_narrow.cuh"
 #include "fp8_rows.cuh"
+#include "fp8_wide.cuh"
 
 namespace sk {
 
@@ -131,6 +132,7 @@ int with_type(int t, F&& fn) {
 
 // ---------------------------------------------------------------- products
 struct Choice {
+  bool wide;                            // rows on the tensor memory's lanes (fp8_wide.cuh), else features (fp8_narrow.cuh)
   int row_tile, feature_tile, split;
   int64_t ctas;
 };
@@ -139,13 +141,17 @@ struct Choice {
 Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, int sms) {
   Choice c;
   const int64_t rows = ceil_div(M, experts);       // of a group, on average
-  c.feature_tile = 128;
-  c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || silu ? 64 : 128;
-  if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(silu && forced > 64 ? 64 : forced);
+  c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  c.wide = rows > 64;
+  if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) {
+    c.row_tile = static_cast<int>(std::min<int64_t>(forced, 128));
+    c.wide = forced > 128 || (silu && forced > 64);
+  }
+  c.feature_tile = c.wide && !silu ? 256 : 128;
   const int64_t n_tiles = ceil_div(N, c.feature_tile);
   const int64_t tiles = (grouped ? ceil_div(M, c.row_tile) + std::min(experts, M) : ceil_div(M, c.row_tile)) * n_tiles;
   c.split = 1;
-  if (!grouped) {
+  if (!grouped && !c.wide) {
     const int64_t kb = ceil_div(K, 128);
     while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * 4) c.split *= 2;
     if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
@@ -170,8 +176,19 @@ int launch_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int
 }
 
 template <bool E8M0, bool SILU>
+int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+  using T = Fp8WideTraits<SILU>;
+  auto kern = fp8_wide_kernel<E8M0, SILU>;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::dynamic_bytes(kFp8MaxExperts)); e != cudaSuccess)
+    return cuda_status(e);
+  LaunchConfig lc(std::min<int64_t>(tiles, dev.sms), 1, T::kThreads, T::dynamic_bytes(p.experts), dependent, 1, stream);
+  return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
+}
+
+template <bool E8M0, bool SILU>
 int launch_product(const Choice& c, const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev,
                    bool dependent, cudaStream_t stream) {
+  if (c.wide) return launch_wide<E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
   switch (c.row_tile) {
     case 16: return launch_narrow<16, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
     case 32: return launch_narrow<32, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
@@ -541,7 +558,7 @@ int sk_fp8_set_option(int key, int64_t value) {
   if (value < 0) return SK_ERR_BAD_ARGUMENT;
   switch (key) {
     case SK_FP8_OPT_ROW_TILE:
-      if (value != 0 && value != 16 && value != 32 && value != 64 && value != 128) return SK_ERR_BAD_ARGUMENT;
+      if (value != 0 && value != 16 && value != 32 && value != 64 && value != 128 && value != 256) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_SPLIT_K:
       if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return SK_ERR_BAD_ARGUMENT;

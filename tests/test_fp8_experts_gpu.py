@@ -5,6 +5,7 @@ import torch
 
 import fp8_util as F
 import slimkernels_b200.torch as sk
+from slimkernels_b200 import capi
 
 pytestmark = pytest.mark.gpu
 E8M0, F32 = torch.float8_e8m0fnu, torch.float32
@@ -181,6 +182,22 @@ def test_expert_layers(T, E, k, hidden, inter, dtype, scales):
     assert y.shape == (T, hidden) and y.dtype == (torch.bfloat16 if dtype == torch.bfloat16 else torch.float16)
     _check_experts(x, routing.rows, routing.weights, routing.offsets, gu, dn, y)
     assert torch.equal(y, sk.fp8_experts(x, routing, *gu, *dn))
+
+
+@pytest.mark.parametrize("row_tile", [16, 32, 64, 256])
+@pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32)])
+def test_expert_layers_every_tile(row_tile, hidden, inter, scales):
+    T, E, k = 300, 5, 2
+    g, gu, dn = _layers(E, hidden, inter, scales, 21)
+    x = F.random_rows(g, T, hidden, torch.bfloat16)
+    routing = sk.route_tokens(torch.randn(T, E, generator=g, device="cuda"), k)
+    lib = capi.load()
+    try:
+        assert lib.sk_fp8_set_option(capi.SK_FP8_OPT_ROW_TILE, row_tile) == 0
+        y = sk.fp8_experts(x, routing, *gu, *dn)
+    finally:
+        lib.sk_fp8_set_option(capi.SK_FP8_OPT_ROW_TILE, 0)
+    _check_experts(x, routing.rows, routing.weights, routing.offsets, gu, dn, y)
 
 
 def test_expert_layers_are_their_parts():

@@ -158,7 +158,7 @@ def test_product_at_working_sizes(M, N, K, scales):
     _check_product(*_operands(M, N, K, scales, M + N + K), torch.bfloat16)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("row_tile", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 2048), (130, 200, 1100), (257, 1024, 1024)])
 def test_every_tile_and_split(M, N, K, row_tile, split, forced):
@@ -301,7 +301,7 @@ def test_grouped_product(offsets, N, K, scales, out_dtype):
     _check_grouped(offsets, offsets[-1] + 9, N, K, scales, out_dtype)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("row_tile", [16, 32, 64, 128, 256])
 def test_grouped_product_every_tile(row_tile, forced):
     forced(row_tile)
     _check_grouped([0, 130, 130, 131, 300, 420, 433], 440, 384, 400, E8M0, torch.float16)
