@@ -77,7 +77,8 @@ SIGNATURES = {
 # The FP8 products of include/sk_fp8.h (same library)
 SK_SCALE_F32, SK_SCALE_E8M0 = 0, 1
 SK_FLOAT_F16, SK_FLOAT_BF16, SK_FLOAT_F32 = 0, 1, 2
-SK_FP8_OPT_ROW_TILE, SK_FP8_OPT_SPLIT_K, SK_FP8_OPT_WAIT_LIMIT_CYCLES, SK_FP8_OPT_TEST_SKIP_COPY = 1, 2, 3, 4
+SK_FP8_OPT_ROW_TILE, SK_FP8_OPT_SPLIT_K, SK_FP8_OPT_WAIT_LIMIT_CYCLES, SK_FP8_OPT_TEST_SKIP_COPY, SK_FP8_OPT_KERNEL = 1, 2, 3, 4, 5
+FP8_NARROW, FP8_WIDE, FP8_SCALED, FP8_SCALED_PAIR = 1, 2, 3, 4
 
 
 class Fp8Rows(ctypes.Structure):
@@ -103,7 +104,7 @@ FP8_SIGNATURES = {
     "sk_fp8_experts_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "sk_fp8_experts": (_int, [_i64, _i64, _vp, _int, _i64, _vp, _vp, _vp, _weight, _weight, _int, _vp, _i64, _int, _vp, _i64, _vp]),
     "sk_fp8_last_device_status": (_int, [_int, ctypes.POINTER(_int)]),
-    "sk_fp8_query_launch": (_int, [_i64, _i64, _i64, _i64, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int)]),
+    "sk_fp8_query_launch": (_int, [_i64, _i64, _i64, _i64, _int, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int)]),
     "sk_fp8_set_option": (_int, [_int, _i64]),
 }
 

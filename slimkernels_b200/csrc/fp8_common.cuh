@@ -34,6 +34,7 @@ struct Fp8Params {
   int up_row0;                          // SiLU epilogue: the up projection's first row / scale block within an expert
   int up_block0;
   int out_bf16;
+  int x_scale_groups, w_scale_groups;   // the scales of four K blocks may be loaded at once (side by side and aligned)
   int vector_out;                       // 16-byte stores are allowed
   int early_weights;                    // the weights may be read before the previous kernel is complete
   int split;                            // CTAs of a cluster that share the K range of a tile
@@ -43,16 +44,59 @@ struct Fp8Params {
 };
 
 // A scale as a float.  8-bit scales are exponents: 2^(b - 127), 255 is NaN.
+__device__ __forceinline__ float scale_of_exponent(uint32_t b) {
+  return __uint_as_float(b == 255u ? 0x7fc00000u : b == 0u ? 0x00400000u : b << 23);
+}
 template <bool E8M0>
 __device__ __forceinline__ float load_scale(const void* base, long long i) {
   if constexpr (E8M0) {
     uint32_t b;
     asm volatile("ld.global.u8 %0, [%1];" : "=r"(b) : "l"(static_cast<const uint8_t*>(base) + i) : "memory");
-    return __uint_as_float(b == 255u ? 0x7fc00000u : b == 0u ? 0x00400000u : b << 23);
+    return scale_of_exponent(b);
   } else {
     return ld_global_f32(static_cast<const float*>(base) + i);
   }
 }
+
+// The scales of up to four K blocks from element i on, `left` of which exist, as they lie in memory: nothing waits for the loads
+// before the first value() (where they cannot be had at once, 8-bit ones are put together on arrival).
+template <bool E8M0>
+struct Scales4 {
+  float f[4];
+  __device__ __forceinline__ void load(const void* base, long long i, long long step, int left, bool whole) {
+    if (whole && left >= 4) {
+      asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                   : "l"(static_cast<const float*>(base) + i) : "memory");
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = j < left ? ld_global_f32(static_cast<const float*>(base) + i + j * step) : 0.f;
+  }
+  // Keeps the loads' first use from being moved up to them (measured: a stall of a load's latency, 900 cycles, every four K blocks).
+  __device__ __forceinline__ void arrive() { asm volatile("" : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3])); }
+  __device__ __forceinline__ float value(int j) const { return f[j]; }
+};
+template <>
+struct Scales4<true> {
+  uint32_t w;
+  __device__ __forceinline__ void load(const void* base, long long i, long long step, int left, bool whole) {
+    const uint8_t* p = static_cast<const uint8_t*>(base) + i;
+    if (whole && left >= 4) {
+      asm volatile("ld.global.b32 %0, [%1];" : "=r"(w) : "l"(p) : "memory");
+      return;
+    }
+    w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) {
+        uint32_t b;
+        asm volatile("ld.global.u8 %0, [%1];" : "=r"(b) : "l"(p + j * step) : "memory");
+        w |= b << (8 * j);
+      }
+  }
+  __device__ __forceinline__ void arrive() { asm volatile("" : "+r"(w)); }
+  __device__ __forceinline__ float value(int j) const { return scale_of_exponent((w >> (8 * j)) & 0xffu); }
+};
 
 // The exponent e of a block's scale 2^e: the smallest with amax <= 448 * 2^e, from amax's bits (448 = 1.75 * 2^8); 0 for an
 // all-zero block, never below -126, so that the scale is a normal float.
@@ -106,6 +150,11 @@ struct GroupTable {
 };
 __host__ __device__ constexpr int group_table_bytes(int experts) { return 2 * (experts + 1) * 4; }
 
+__device__ __forceinline__ float lds_f32(uint32_t addr) {   // stays where it is
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ int ld_global_int(const int* p) {
   int v;
   asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");

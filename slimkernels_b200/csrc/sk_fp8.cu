@@ -9,6 +9,7 @@
 #include "fp8_common.cuh"
 #include "fp8_narrow.cuh"
 #include "fp8_rows.cuh"
+#include "fp8_scaled.cuh"
 #include "fp8_wide.cuh"
 
 namespace sk {
@@ -17,7 +18,7 @@ __device__ int g_fp8_status;            // the first wait that ran into its limi
 
 namespace {
 
-std::atomic<int64_t> g_options[5];
+std::atomic<int64_t> g_options[6];
 
 int cuda_status(cudaError_t e) {
   if (e == cudaSuccess) return SK_OK;
@@ -132,26 +133,29 @@ int with_type(int t, F&& fn) {
 
 // ---------------------------------------------------------------- products
 struct Choice {
-  bool wide;                            // rows on the tensor memory's lanes (fp8_wide.cuh), else features (fp8_narrow.cuh)
+  int kernel;                           // sk_fp8_kernel
   int row_tile, feature_tile, split;
   int64_t ctas;
 };
 
 // One product, or the products of a group: what decides how it is launched.
-Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, int sms) {
+Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, int sms) {
   Choice c;
   const int64_t rows = ceil_div(M, experts);       // of a group, on average
-  c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  c.wide = rows > 64;
-  if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) {
-    c.row_tile = static_cast<int>(std::min<int64_t>(forced, 128));
-    c.wide = forced > 128 || (silu && forced > 64);
+  c.kernel = rows <= 64 ? SK_FP8_KERNEL_NARROW : e8m0 ? SK_FP8_KERNEL_SCALED_PAIR : SK_FP8_KERNEL_WIDE;
+  if (const int64_t forced = g_options[SK_FP8_OPT_KERNEL].load()) c.kernel = !e8m0 && forced > SK_FP8_KERNEL_WIDE ? SK_FP8_KERNEL_WIDE : static_cast<int>(forced);
+  if (c.kernel == SK_FP8_KERNEL_NARROW) {
+    c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || silu ? 64 : 128;
+    if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(std::min<int64_t>(forced, silu ? 64 : 128));
+    c.feature_tile = 128;
+  } else {
+    c.row_tile = c.kernel == SK_FP8_KERNEL_SCALED_PAIR ? 256 : 128;
+    c.feature_tile = silu ? 128 : 256;
   }
-  c.feature_tile = c.wide && !silu ? 256 : 128;
   const int64_t n_tiles = ceil_div(N, c.feature_tile);
   const int64_t tiles = (grouped ? ceil_div(M, c.row_tile) + std::min(experts, M) : ceil_div(M, c.row_tile)) * n_tiles;
   c.split = 1;
-  if (!grouped && !c.wide) {
+  if (!grouped && c.kernel == SK_FP8_KERNEL_NARROW) {
     const int64_t kb = ceil_div(K, 128);
     while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * 4) c.split *= 2;
     if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
@@ -185,10 +189,24 @@ int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
+template <int CTAS, bool SILU>
+int launch_scaled(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+  using T = Fp8ScaledTraits<CTAS, SILU>;
+  auto kern = fp8_scaled_kernel<CTAS, SILU>;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::dynamic_bytes(kFp8MaxExperts)); e != cudaSuccess)
+    return cuda_status(e);
+  LaunchConfig lc(std::min<int64_t>(tiles, dev.sms / CTAS) * CTAS, 1, T::kThreads, T::dynamic_bytes(p.experts), dependent, CTAS, stream);
+  return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
+}
+
 template <bool E8M0, bool SILU>
 int launch_product(const Choice& c, const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev,
                    bool dependent, cudaStream_t stream) {
-  if (c.wide) return launch_wide<E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+  if (c.kernel == SK_FP8_KERNEL_WIDE) return launch_wide<E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+  if constexpr (E8M0) {
+    if (c.kernel == SK_FP8_KERNEL_SCALED) return launch_scaled<1, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+    if (c.kernel == SK_FP8_KERNEL_SCALED_PAIR) return launch_scaled<2, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+  }
   switch (c.row_tile) {
     case 16: return launch_narrow<16, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
     case 32: return launch_narrow<32, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
@@ -208,7 +226,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   const int64_t N = w->N, K = w->K;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
-  const Choice c = choose(M, N, K, experts, offsets != nullptr, silu, dev.sms);
+  const Choice c = choose(M, N, K, experts, offsets != nullptr, silu, scale_type == SK_SCALE_E8M0, dev.sms);
   Fp8Params p = {};
   p.x_scale = x->scale;
   p.xs_row = x->scale_row;
@@ -234,6 +252,9 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   p.n_tiles = static_cast<int>(ceil_div(N, c.feature_tile));
   p.out_bf16 = out_dtype == SK_OUT_BF16;
   p.vector_out = !silu && aligned(out, 16) && ld_out % 8 == 0;
+  const int64_t four = 4 * scale_bytes(scale_type);
+  p.x_scale_groups = p.xs_blk == 1 && p.xs_row % 4 == 0 && aligned(p.x_scale, four);
+  p.w_scale_groups = p.k_blocks % 4 == 0 && aligned(p.w_scale, four);
   p.early_weights = early_weights && offsets == nullptr;
   p.split = c.split;
   p.skip_block = static_cast<int>(g_options[SK_FP8_OPT_TEST_SKIP_COPY].load()) - 1;
@@ -244,7 +265,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   if (tiles > kIntMax / 8) return SK_ERR_BAD_SHAPE;
   CUtensorMap mw, mx;
   if (int rc = codes_map(w->q, w->experts * N, K, w->ld, 128, &mw); rc != SK_OK) return rc;
-  if (int rc = codes_map(x->q, M, K, x->ld, c.row_tile, &mx); rc != SK_OK) return rc;
+  if (int rc = codes_map(x->q, M, K, x->ld, std::min(c.row_tile, 128), &mx); rc != SK_OK) return rc;
   return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
     return with_bool(silu, [&](auto s) {
       return launch_product<decltype(e8m0)::value, decltype(s)::value>(c, mw, mx, p, tiles, dev, dependent, stream);
@@ -542,11 +563,13 @@ int sk_fp8_last_device_status(int device, int* device_status) {
   return word == 0 ? SK_OK : SK_ERR_DEVICE_TIMEOUT;
 }
 
-int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int* row_tile, int* feature_tile, int* split, int* ctas) {
+int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int scale_type, int* kernel, int* row_tile, int* feature_tile, int* split, int* ctas) {
   if (M < 1 || N < 1 || K < 1 || experts < 1 || experts > kFp8MaxExperts) return SK_ERR_BAD_SHAPE;
+  if (!is_scale_type(scale_type)) return SK_ERR_BAD_ARGUMENT;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
-  const Choice c = choose(M, N, K, experts, experts > 1, false, dev.sms);
+  const Choice c = choose(M, N, K, experts, experts > 1, false, scale_type == SK_SCALE_E8M0, dev.sms);
+  if (kernel) *kernel = c.kernel;
   if (row_tile) *row_tile = c.row_tile;
   if (feature_tile) *feature_tile = c.feature_tile;
   if (split) *split = c.split;
@@ -558,13 +581,16 @@ int sk_fp8_set_option(int key, int64_t value) {
   if (value < 0) return SK_ERR_BAD_ARGUMENT;
   switch (key) {
     case SK_FP8_OPT_ROW_TILE:
-      if (value != 0 && value != 16 && value != 32 && value != 64 && value != 128 && value != 256) return SK_ERR_BAD_ARGUMENT;
+      if (value != 0 && value != 16 && value != 32 && value != 64 && value != 128) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_SPLIT_K:
       if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_WAIT_LIMIT_CYCLES:
       if (value != 0 && value < 1000) return SK_ERR_BAD_ARGUMENT;
+      break;
+    case SK_FP8_OPT_KERNEL:
+      if (value > SK_FP8_KERNEL_SCALED_PAIR) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_TEST_SKIP_COPY:
       if (value > kIntMax) return SK_ERR_BAD_ARGUMENT;

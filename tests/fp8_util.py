@@ -1,11 +1,14 @@
 """The FP8 operators by their definition, in 64 bits, and how far a kernel's result may be from it.
 
 A product's tolerance.  Codes are exact, products of two e4m3 values too; what is rounded is
-  * every addition: at most 128 inside a block and one per block outside, each off by at most 2^-23 (an addition that truncates) of
-    the absolute sum S = sum_k |x w|; the product of the two scales and the product with it: 3 * 2^-24 of S at most,
+  * every addition, off by at most 2^-23 (an addition that truncates) of the absolute sum S = sum_k |x w| it adds to.  Kernels that
+    scale every K block's sum in fp32: at most 128 additions inside a block and one per block outside; the product of the two scales
+    and the product with it are off by 3 * 2^-24 of S at most.  Kernels that leave the scales to the tensor core: each of the K / 32 MMAs
+    adds to one accumulator, and inside an MMA 32 products meet, whose roundings are relative to that MMA's share of S.  So
+    128 + K / 32 + 2 covers both,
   * the result to its 16-bit type: half a step, 2^-8 (bf16) or 2^-11 (fp16) of its value, and 2^-25 absolutely where fp16 has
     subnormals (bf16's lie below everything here).
-So |y - exact| <= (128 + blocks + 2) 2^-23 S + half * (|exact| + that) + 2^-25.
+So |y - exact| <= (128 + K / 32 + 2) 2^-23 S + half * (|exact| + that) + 2^-25.
 """
 import numpy as np
 import torch
@@ -75,10 +78,14 @@ def quantised_values(x):
     return q * pow2(e).repeat_interleave(BLOCK, dim=1)[:, :x.shape[1]]
 
 
+def sum_roundings(K):
+    return 128 + ceil_div(K, 32) + 2
+
+
 def product_tolerance(xv, wv, out_dtype):
     """(exact, tolerance) of xv @ wv.T for values xv [M, K], wv [N, K] in float64."""
     exact = xv @ wv.T
-    acc = (128 + ceil_div(xv.shape[1], BLOCK) + 2) * 2.0 ** -23 * (xv.abs() @ wv.abs().T)
+    acc = sum_roundings(xv.shape[1]) * 2.0 ** -23 * (xv.abs() @ wv.abs().T)
     if out_dtype is None:
         return exact, acc
     half = HALF_STEP[out_dtype]

@@ -152,7 +152,7 @@ def _check_experts(x, rows, weights, offsets, gu, dn, y):
         lo, hi = _quantised_interval(h - dh, h + dh)
         w = F.weight_values(dn[0][e], dn[1][e])
         mid, rad = _interval_product(lo, hi, w)
-        acc = (128 + F.ceil_div(w.shape[1], 128) + 2) * 2.0 ** -23 * (torch.maximum(lo.abs(), hi.abs()) @ w.abs().T)
+        acc = F.sum_roundings(w.shape[1]) * 2.0 ** -23 * (torch.maximum(lo.abs(), hi.abs()) @ w.abs().T)
         dy = rad + acc
         dy = dy + half * (mid.abs() + dy) + 2.0 ** -25
         wt = weights[t, j][:, None]
@@ -184,18 +184,20 @@ def test_expert_layers(T, E, k, hidden, inter, dtype, scales):
     assert torch.equal(y, sk.fp8_experts(x, routing, *gu, *dn))
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 256])
-@pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32)])
-def test_expert_layers_every_tile(row_tile, hidden, inter, scales):
-    T, E, k = 300, 5, 2
+@pytest.mark.parametrize("kernel,row_tile", [(capi.FP8_NARROW, 16), (capi.FP8_NARROW, 32), (capi.FP8_NARROW, 64), (capi.FP8_WIDE, 0),
+                                             (capi.FP8_SCALED, 0), (capi.FP8_SCALED_PAIR, 0)])
+@pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32), (272, 144, E8M0)])
+def test_expert_layers_every_kernel(kernel, row_tile, hidden, inter, scales):
+    T, E, k = 500, 5, 2
     g, gu, dn = _layers(E, hidden, inter, scales, 21)
     x = F.random_rows(g, T, hidden, torch.bfloat16)
     routing = sk.route_tokens(torch.randn(T, E, generator=g, device="cuda"), k)
     lib = capi.load()
     try:
-        assert lib.sk_fp8_set_option(capi.SK_FP8_OPT_ROW_TILE, row_tile) == 0
+        assert lib.sk_fp8_set_option(capi.SK_FP8_OPT_KERNEL, kernel) == 0 and lib.sk_fp8_set_option(capi.SK_FP8_OPT_ROW_TILE, row_tile) == 0
         y = sk.fp8_experts(x, routing, *gu, *dn)
     finally:
+        lib.sk_fp8_set_option(capi.SK_FP8_OPT_KERNEL, 0)
         lib.sk_fp8_set_option(capi.SK_FP8_OPT_ROW_TILE, 0)
     _check_experts(x, routing.rows, routing.weights, routing.offsets, gu, dn, y)
 

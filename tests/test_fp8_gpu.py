@@ -26,10 +26,10 @@ def _no_wait_expired():
     assert sk.fp8_device_status() == 0
 
 
-def _options(row_tile=0, split=0, limit=0, skip=0):
+def _options(row_tile=0, split=0, limit=0, skip=0, kernel=0):
     lib = capi.load()
     for key, value in ((capi.SK_FP8_OPT_ROW_TILE, row_tile), (capi.SK_FP8_OPT_SPLIT_K, split), (capi.SK_FP8_OPT_WAIT_LIMIT_CYCLES, limit),
-                       (capi.SK_FP8_OPT_TEST_SKIP_COPY, skip)):
+                       (capi.SK_FP8_OPT_TEST_SKIP_COPY, skip), (capi.SK_FP8_OPT_KERNEL, kernel)):
         assert lib.sk_fp8_set_option(key, value) == 0
 
 
@@ -158,14 +158,45 @@ def test_product_at_working_sizes(M, N, K, scales):
     _check_product(*_operands(M, N, K, scales, M + N + K), torch.bfloat16)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 2048), (130, 200, 1100), (257, 1024, 1024)])
-def test_every_tile_and_split(M, N, K, row_tile, split, forced):
-    forced(row_tile, split)
+def test_narrow_kernel_every_tile_and_split(M, N, K, row_tile, split, forced):
+    forced(row_tile, split, kernel=capi.FP8_NARROW)
     x = _operands(M, N, K, E8M0, 3)
     y = _check_product(*x, torch.float16)
     assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
+
+
+KERNELS = [(capi.FP8_WIDE, F32), (capi.FP8_WIDE, E8M0), (capi.FP8_SCALED, E8M0), (capi.FP8_SCALED_PAIR, E8M0)]
+
+
+@pytest.mark.parametrize("kernel,scales", KERNELS)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 128, 2048), (130, 200, 1100), (128, 256, 128), (257, 1030, 1024), (300, 513, 400), (600, 8000, 640),
+                                   (5000, 2560, 300)])
+def test_kernels_for_many_rows(M, N, K, kernel, scales, forced):
+    forced(kernel=kernel)
+    x = _operands(M, N, K, scales, 3)
+    y = _check_product(*x, torch.float16)
+    assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
+
+
+@pytest.mark.parametrize("kernel", [capi.FP8_SCALED, capi.FP8_SCALED_PAIR])
+def test_every_scale_reaches_its_row_and_block(kernel, forced):
+    """Scales that differ from row to row and block to block by large factors, in any memory order: none may be taken for another's."""
+    forced(kernel=kernel)
+    M, N, K = 300, 700, 1500
+    x_q, x_s, w_q, w_s = _operands(M, N, K, E8M0, 4)
+    g = F.generator(5)
+    x_s.view(torch.uint8)[...] = torch.randint(100, 150, x_s.shape, generator=g, device="cuda").to(torch.uint8)
+    w_s.view(torch.uint8)[...] = torch.randint(100, 150, w_s.shape, generator=g, device="cuda").to(torch.uint8)
+    y = _check_product(x_q, x_s, w_q, w_s, torch.bfloat16)
+    turned = x_s.view(torch.uint8).t().contiguous().t().view(E8M0)
+    wide = torch.zeros(M, 13, dtype=torch.uint8, device="cuda")
+    wide[:, 1:] = x_s.view(torch.uint8)
+    assert turned.stride() == (1, M)
+    for other in (turned, wide[:, 1:].view(E8M0)):
+        assert torch.equal(y, sk.fp8_gemm(x_q, other, w_q, w_s))
 
 
 def test_product_strides():
@@ -187,9 +218,10 @@ def test_product_strides():
     assert sk.fp8_gemm(x_q[:0], x_s[:0], w_q, w_s).shape == (0, 200)
 
 
-@pytest.mark.parametrize("scales", [E8M0, F32])
+@pytest.mark.parametrize("kernel,scales", [(0, E8M0), (0, F32)] + KERNELS)
 @pytest.mark.parametrize("M", [3, 40, 200])
-def test_nan_stays_in_its_row_and_feature(M, scales):
+def test_nan_stays_in_its_row_and_feature(M, kernel, scales, forced):
+    forced(kernel=kernel)
     g = F.generator(M)
     x = F.random_rows(g, M, 600)
     w = torch.randn(300, 600, generator=g, device="cuda")
@@ -204,11 +236,13 @@ def test_nan_stays_in_its_row_and_feature(M, scales):
     assert not bool(nan.any())
 
 
-def test_scales_at_the_ends_of_their_range():
+@pytest.mark.parametrize("kernel", [0, capi.FP8_WIDE, capi.FP8_SCALED, capi.FP8_SCALED_PAIR])
+def test_scales_at_the_ends_of_their_range(kernel, forced):
     """2^-127 (the smallest 8-bit scale, a subnormal float) times large ones; a NaN scale; sums that leave the range of fp32.
 
     The sum over the blocks is kept in fp32: where a block's share or the sum up to it is beyond 2^128, it is infinite from there on, or
     NaN once two infinities of either sign meet, whatever the whole sum would be.  There the result has to be not finite."""
+    forced(kernel=kernel)
     x_q, x_s, w_q, w_s = _operands(4, 128, 256, E8M0, 2)
     bits = x_s.view(torch.uint8)
     bits[0], bits[1], bits[2, 0] = 0, 1, 255
@@ -301,10 +335,18 @@ def test_grouped_product(offsets, N, K, scales, out_dtype):
     _check_grouped(offsets, offsets[-1] + 9, N, K, scales, out_dtype)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 128, 256])
-def test_grouped_product_every_tile(row_tile, forced):
-    forced(row_tile)
+@pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
+def test_grouped_product_every_narrow_tile(row_tile, forced):
+    forced(row_tile, kernel=capi.FP8_NARROW)
     _check_grouped([0, 130, 130, 131, 300, 420, 433], 440, 384, 400, E8M0, torch.float16)
+
+
+@pytest.mark.parametrize("kernel,scales", KERNELS)
+@pytest.mark.parametrize("N,K", [(384, 400), (130, 1040)])
+def test_grouped_product_every_kernel(N, K, kernel, scales, forced):
+    forced(kernel=kernel)
+    _check_grouped([2, 130, 130, 131, 300, 700, 713], 720, N, K, scales, torch.float16)
+    _check_grouped([0, 0, 0, 3], 3, N, K, scales, torch.bfloat16)
 
 
 def test_grouped_product_many_experts_and_fresh_result():
@@ -408,16 +450,17 @@ def test_weights_written_on_the_way_are_seen():
     assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
 
 
-@pytest.mark.parametrize("M", [4, 200])
-def test_a_copy_that_never_lands_ends_in_a_status(M, forced):
+@pytest.mark.parametrize("M,kernel", [(4, 0), (200, capi.FP8_NARROW), (200, capi.FP8_WIDE), (200, capi.FP8_SCALED), (500, capi.FP8_SCALED_PAIR)])
+def test_a_copy_that_never_lands_ends_in_a_status(M, kernel, forced):
     x = _operands(M, 256, 1024, E8M0, 3)
+    forced(kernel=kernel)
     want = sk.fp8_gemm(*x)
-    forced(limit=2_000_000, skip=3)
+    forced(limit=2_000_000, skip=3, kernel=kernel)
     sk.fp8_gemm(*x)
     torch.cuda.synchronize()
     assert sk.fp8_device_status() != 0
     assert sk.fp8_device_status() == 0
-    _options()
+    forced(kernel=kernel)
     assert torch.equal(sk.fp8_gemm(*x), want)
 
 
