@@ -95,7 +95,8 @@ typedef enum sk_fp8_kernel {
   SK_FP8_KERNEL_NARROW = 1,     /* few rows: features on the tensor memory's lanes */
   SK_FP8_KERNEL_WIDE = 2,       /* many rows on the lanes, scales applied to every K block's sums in fp32 */
   SK_FP8_KERNEL_SCALED = 3,     /* many rows, 8-bit scales applied by the tensor core */
-  SK_FP8_KERNEL_SCALED_PAIR = 4 /* the same on pairs of CTAs */
+  SK_FP8_KERNEL_SCALED_PAIR = 4, /* the same on pairs of CTAs */
+  SK_FP8_KERNEL_SCALED_NARROW = 5 /* few rows, 8-bit scales applied by the tensor core */
 } sk_fp8_kernel;
 /* The launch a product makes: kernel, rows per tile, features per tile, CTAs that share a tile's K range, CTAs (at most).  experts > 1:
  * a product by expert of M rows in all. */
@@ -108,7 +109,7 @@ typedef enum sk_fp8_option {
   SK_FP8_OPT_SPLIT_K = 2,           /* CTAs that share the K range of a tile (products of one group) */
   SK_FP8_OPT_WAIT_LIMIT_CYCLES = 3, /* as SK_OPT_WAIT_LIMIT_CYCLES */
   SK_FP8_OPT_TEST_SKIP_COPY = 4,    /* as SK_OPT_TEST_SKIP_COPY */
-  SK_FP8_OPT_KERNEL = 5             /* sk_fp8_kernel; with 32-bit scales 3 and 4 mean 2 */
+  SK_FP8_OPT_KERNEL = 5             /* sk_fp8_kernel; with 32-bit scales 3 and 4 mean 2, and 5 means 1 */
 } sk_fp8_option;
 int sk_fp8_set_option(int key, int64_t value);
 

@@ -37,6 +37,7 @@ struct Fp8Params {
   int x_scale_groups, w_scale_groups;   // the scales of four K blocks may be loaded at once (side by side and aligned)
   int vector_out;                       // 16-byte stores are allowed
   int early_weights;                    // the weights may be read before the previous kernel is complete
+  int stages;                           // depth of the ring (kernels whose launch decides it)
   int split;                            // CTAs of a cluster that share the K range of a tile
   int skip_block;                       // failure-path test hook: this K block's copies are left out (-1: off)
   long long wait_limit;

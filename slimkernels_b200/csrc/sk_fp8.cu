@@ -10,6 +10,7 @@
 #include "fp8_narrow.cuh"
 #include "fp8_rows.cuh"
 #include "fp8_scaled.cuh"
+#include "fp8_scaled_narrow.cuh"
 #include "fp8_wide.cuh"
 
 namespace sk {
@@ -142,9 +143,10 @@ struct Choice {
 Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, int sms) {
   Choice c;
   const int64_t rows = ceil_div(M, experts);       // of a group, on average
-  c.kernel = rows <= 64 ? SK_FP8_KERNEL_NARROW : e8m0 ? SK_FP8_KERNEL_SCALED_PAIR : SK_FP8_KERNEL_WIDE;
-  if (const int64_t forced = g_options[SK_FP8_OPT_KERNEL].load()) c.kernel = !e8m0 && forced > SK_FP8_KERNEL_WIDE ? SK_FP8_KERNEL_WIDE : static_cast<int>(forced);
-  if (c.kernel == SK_FP8_KERNEL_NARROW) {
+  c.kernel = rows <= 64 ? (e8m0 ? SK_FP8_KERNEL_SCALED_NARROW : SK_FP8_KERNEL_NARROW) : e8m0 ? SK_FP8_KERNEL_SCALED_PAIR : SK_FP8_KERNEL_WIDE;
+  if (const int64_t forced = g_options[SK_FP8_OPT_KERNEL].load()) c.kernel = e8m0 ? static_cast<int>(forced) : forced == SK_FP8_KERNEL_NARROW || forced == SK_FP8_KERNEL_SCALED_NARROW ? SK_FP8_KERNEL_NARROW : SK_FP8_KERNEL_WIDE;
+  const bool narrow = c.kernel == SK_FP8_KERNEL_NARROW || c.kernel == SK_FP8_KERNEL_SCALED_NARROW;
+  if (narrow) {
     c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || silu ? 64 : 128;
     if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(std::min<int64_t>(forced, silu ? 64 : 128));
     c.feature_tile = 128;
@@ -155,7 +157,7 @@ Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bo
   const int64_t n_tiles = ceil_div(N, c.feature_tile);
   const int64_t tiles = (grouped ? ceil_div(M, c.row_tile) + std::min(experts, M) : ceil_div(M, c.row_tile)) * n_tiles;
   c.split = 1;
-  if (!grouped && c.kernel == SK_FP8_KERNEL_NARROW) {
+  if (!grouped && narrow) {
     const int64_t kb = ceil_div(K, 128);
     while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * 4) c.split *= 2;
     if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
@@ -189,6 +191,23 @@ int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
+// The ring: 3 to 12 stages, for two CTAs per SM where there are more CTAs than SMs and two fit, else for one.
+template <int TOK, bool SILU>
+int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+  using T = Fp8ScaledNarrowTraits<TOK, SILU>;
+  auto kern = fp8_scaled_narrow_kernel<TOK, SILU>;
+  constexpr int kSm = 233472, kCta = 232448;        // shared memory of an SM (1 KiB per CTA goes to the system) and of a CTA
+  const int fixed = T::fixed_bytes(p.split, p.experts);
+  int ctas = T::kCtas == 2 && tiles * p.split > dev.sms ? 2 : 1;
+  if ((kSm / ctas - 1024 - fixed) / T::kStageBytes < 3) ctas = 1;
+  p.stages = std::min(T::kMaxStages, ((ctas == 1 ? kCta : kSm / 2 - 1024) - fixed) / T::kStageBytes);
+  static_assert((kCta - T::fixed_bytes(SILU ? 1 : 8, 1)) / T::kStageBytes >= 3 && (kCta - T::fixed_bytes(1, kFp8MaxExperts)) / T::kStageBytes >= 3, "room for a ring");
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kCta); e != cudaSuccess) return cuda_status(e);
+  const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * ctas);
+  LaunchConfig lc(grid, 1, T::kThreads, fixed + p.stages * T::kStageBytes, dependent, p.split, stream);
+  return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
+}
+
 template <int CTAS, bool SILU>
 int launch_scaled(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
   using T = Fp8ScaledTraits<CTAS, SILU>;
@@ -206,6 +225,16 @@ int launch_product(const Choice& c, const CUtensorMap& mw, const CUtensorMap& mx
   if constexpr (E8M0) {
     if (c.kernel == SK_FP8_KERNEL_SCALED) return launch_scaled<1, SILU>(mw, mx, p, tiles, dev, dependent, stream);
     if (c.kernel == SK_FP8_KERNEL_SCALED_PAIR) return launch_scaled<2, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+    if (c.kernel == SK_FP8_KERNEL_SCALED_NARROW) {
+      switch (c.row_tile) {
+        case 16: return launch_scaled_narrow<16, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+        case 32: return launch_scaled_narrow<32, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+        case 64: return launch_scaled_narrow<64, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+        default:
+          if constexpr (SILU) return SK_ERR_UNAVAILABLE;
+          else return launch_scaled_narrow<128, SILU>(mw, mx, p, tiles, dev, dependent, stream);
+      }
+    }
   }
   switch (c.row_tile) {
     case 16: return launch_narrow<16, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
@@ -590,7 +619,7 @@ int sk_fp8_set_option(int key, int64_t value) {
       if (value != 0 && value < 1000) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_KERNEL:
-      if (value > SK_FP8_KERNEL_SCALED_PAIR) return SK_ERR_BAD_ARGUMENT;
+      if (value > SK_FP8_KERNEL_SCALED_NARROW) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_TEST_SKIP_COPY:
       if (value > kIntMax) return SK_ERR_BAD_ARGUMENT;

@@ -185,7 +185,8 @@ def test_expert_layers(T, E, k, hidden, inter, dtype, scales):
 
 
 @pytest.mark.parametrize("kernel,row_tile", [(capi.FP8_NARROW, 16), (capi.FP8_NARROW, 32), (capi.FP8_NARROW, 64), (capi.FP8_WIDE, 0),
-                                             (capi.FP8_SCALED, 0), (capi.FP8_SCALED_PAIR, 0)])
+                                             (capi.FP8_SCALED, 0), (capi.FP8_SCALED_PAIR, 0), (capi.FP8_SCALED_NARROW, 16),
+                                             (capi.FP8_SCALED_NARROW, 32), (capi.FP8_SCALED_NARROW, 64)])
 @pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32), (272, 144, E8M0)])
 def test_expert_layers_every_kernel(kernel, row_tile, hidden, inter, scales):
     T, E, k = 500, 5, 2

@@ -161,30 +161,34 @@ def test_product_at_working_sizes(M, N, K, scales):
 @pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 2048), (130, 200, 1100), (257, 1024, 1024)])
-def test_narrow_kernel_every_tile_and_split(M, N, K, row_tile, split, forced):
-    forced(row_tile, split, kernel=capi.FP8_NARROW)
-    x = _operands(M, N, K, E8M0, 3)
+@pytest.mark.parametrize("kernel,scales", [(capi.FP8_NARROW, E8M0), (capi.FP8_NARROW, F32), (capi.FP8_SCALED_NARROW, E8M0)])
+def test_kernels_for_few_rows_every_tile_and_split(M, N, K, kernel, scales, row_tile, split, forced):
+    forced(row_tile, split, kernel=kernel)
+    x = _operands(M, N, K, scales, 3)
     y = _check_product(*x, torch.float16)
     assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
 
 
-KERNELS = [(capi.FP8_WIDE, F32), (capi.FP8_WIDE, E8M0), (capi.FP8_SCALED, E8M0), (capi.FP8_SCALED_PAIR, E8M0)]
+KERNELS = [(capi.FP8_WIDE, F32), (capi.FP8_WIDE, E8M0), (capi.FP8_SCALED, E8M0), (capi.FP8_SCALED_PAIR, E8M0), (capi.FP8_SCALED_NARROW, E8M0)]
 
 
 @pytest.mark.parametrize("kernel,scales", KERNELS)
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 128, 2048), (130, 200, 1100), (128, 256, 128), (257, 1030, 1024), (300, 513, 400), (600, 8000, 640),
                                    (5000, 2560, 300)])
-def test_kernels_for_many_rows(M, N, K, kernel, scales, forced):
+def test_every_kernel(M, N, K, kernel, scales, forced):
     forced(kernel=kernel)
     x = _operands(M, N, K, scales, 3)
     y = _check_product(*x, torch.float16)
     assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
 
 
-@pytest.mark.parametrize("kernel", [capi.FP8_SCALED, capi.FP8_SCALED_PAIR])
-def test_every_scale_reaches_its_row_and_block(kernel, forced):
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
+@pytest.mark.parametrize("kernel", [capi.FP8_SCALED, capi.FP8_SCALED_PAIR, capi.FP8_SCALED_NARROW])
+def test_every_scale_reaches_its_row_and_block(kernel, row_tile, forced):
     """Scales that differ from row to row and block to block by large factors, in any memory order: none may be taken for another's."""
-    forced(kernel=kernel)
+    if row_tile and kernel != capi.FP8_SCALED_NARROW:
+        pytest.skip("the row tile is the narrow kernel's")
+    forced(row_tile, kernel=kernel)
     M, N, K = 300, 700, 1500
     x_q, x_s, w_q, w_s = _operands(M, N, K, E8M0, 4)
     g = F.generator(5)
@@ -236,7 +240,7 @@ def test_nan_stays_in_its_row_and_feature(M, kernel, scales, forced):
     assert not bool(nan.any())
 
 
-@pytest.mark.parametrize("kernel", [0, capi.FP8_WIDE, capi.FP8_SCALED, capi.FP8_SCALED_PAIR])
+@pytest.mark.parametrize("kernel", [0, capi.FP8_NARROW, capi.FP8_WIDE, capi.FP8_SCALED, capi.FP8_SCALED_PAIR])
 def test_scales_at_the_ends_of_their_range(kernel, forced):
     """2^-127 (the smallest 8-bit scale, a subnormal float) times large ones; a NaN scale; sums that leave the range of fp32.
 
@@ -336,8 +340,9 @@ def test_grouped_product(offsets, N, K, scales, out_dtype):
 
 
 @pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
-def test_grouped_product_every_narrow_tile(row_tile, forced):
-    forced(row_tile, kernel=capi.FP8_NARROW)
+@pytest.mark.parametrize("kernel", [capi.FP8_NARROW, capi.FP8_SCALED_NARROW])
+def test_grouped_product_every_narrow_tile(kernel, row_tile, forced):
+    forced(row_tile, kernel=kernel)
     _check_grouped([0, 130, 130, 131, 300, 420, 433], 440, 384, 400, E8M0, torch.float16)
 
 
@@ -450,7 +455,7 @@ def test_weights_written_on_the_way_are_seen():
     assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
 
 
-@pytest.mark.parametrize("M,kernel", [(4, 0), (200, capi.FP8_NARROW), (200, capi.FP8_WIDE), (200, capi.FP8_SCALED), (500, capi.FP8_SCALED_PAIR)])
+@pytest.mark.parametrize("M,kernel", [(4, 0), (4, capi.FP8_NARROW), (200, capi.FP8_NARROW), (200, capi.FP8_SCALED_NARROW), (200, capi.FP8_WIDE), (200, capi.FP8_SCALED), (500, capi.FP8_SCALED_PAIR)])
 def test_a_copy_that_never_lands_ends_in_a_status(M, kernel, forced):
     x = _operands(M, 256, 1024, E8M0, 3)
     forced(kernel=kernel)
