@@ -92,12 +92,10 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
  * non-zero maps to SK_ERR_DEVICE_TIMEOUT.  sk_device_status_string words it.  The output of such a launch is undefined. */
 int sk_fp8_last_device_status(int device, int* device_status);
 typedef enum sk_fp8_kernel {
-  SK_FP8_KERNEL_NARROW = 1,     /* few rows: features on the tensor memory's lanes */
-  SK_FP8_KERNEL_WIDE = 2,       /* many rows on the lanes, scales applied to every K block's sums in fp32 */
-  SK_FP8_KERNEL_SCALED = 3,     /* many rows, 8-bit scales applied by the tensor core */
-  SK_FP8_KERNEL_SCALED_PAIR = 4, /* the same on pairs of CTAs */
-  SK_FP8_KERNEL_SCALED_NARROW = 5 /* few rows, 8-bit scales applied by the tensor core */
-} sk_fp8_kernel;
+  SK_FP8_KERNEL_FEW = 1,        /* few rows: features on the tensor memory's lanes, tiles of 16, 32 or (8-bit scales) 64 rows */
+  SK_FP8_KERNEL_MANY = 2,       /* many rows: 128 of them on the lanes */
+  SK_FP8_KERNEL_PAIR = 3        /* the same on pairs of CTAs, 256 rows (8-bit scales) */
+} sk_fp8_kernel;                /* 8-bit scales are multiplied in by the tensor core, 32-bit ones in fp32 after every K block */
 /* The launch a product makes: kernel, rows per tile, features per tile, CTAs that share a tile's K range, CTAs (at most).  experts > 1:
  * a product by expert of M rows in all. */
 int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int scale_type, int* kernel, int* row_tile, int* feature_tile,
@@ -105,11 +103,11 @@ int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int sc
 
 /* Testing and tuning, process-wide; 0 restores the default. */
 typedef enum sk_fp8_option {
-  SK_FP8_OPT_ROW_TILE = 1,          /* rows per tile of the kernel for few rows: 16 / 32 / 64 / 128 */
+  SK_FP8_OPT_ROW_TILE = 1,          /* rows per tile of the kernel for few rows: 16 / 32 / 64 (32 where there is no 64) */
   SK_FP8_OPT_SPLIT_K = 2,           /* CTAs that share the K range of a tile (products of one group) */
   SK_FP8_OPT_WAIT_LIMIT_CYCLES = 3, /* as SK_OPT_WAIT_LIMIT_CYCLES */
   SK_FP8_OPT_TEST_SKIP_COPY = 4,    /* as SK_OPT_TEST_SKIP_COPY */
-  SK_FP8_OPT_KERNEL = 5             /* sk_fp8_kernel; with 32-bit scales 3 and 4 mean 2, and 5 means 1 */
+  SK_FP8_OPT_KERNEL = 5             /* sk_fp8_kernel; with 32-bit scales 3 means 2 */
 } sk_fp8_option;
 int sk_fp8_set_option(int key, int64_t value);
 

@@ -78,7 +78,7 @@ SIGNATURES = {
 SK_SCALE_F32, SK_SCALE_E8M0 = 0, 1
 SK_FLOAT_F16, SK_FLOAT_BF16, SK_FLOAT_F32 = 0, 1, 2
 SK_FP8_OPT_ROW_TILE, SK_FP8_OPT_SPLIT_K, SK_FP8_OPT_WAIT_LIMIT_CYCLES, SK_FP8_OPT_TEST_SKIP_COPY, SK_FP8_OPT_KERNEL = 1, 2, 3, 4, 5
-FP8_NARROW, FP8_WIDE, FP8_SCALED, FP8_SCALED_PAIR, FP8_SCALED_NARROW = 1, 2, 3, 4, 5
+FP8_FEW, FP8_MANY, FP8_PAIR = 1, 2, 3
 
 
 class Fp8Rows(ctypes.Structure):

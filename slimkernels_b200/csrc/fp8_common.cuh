@@ -44,60 +44,33 @@ struct Fp8Params {
   int* status;
 };
 
-// A scale as a float.  8-bit scales are exponents: 2^(b - 127), 255 is NaN.
-__device__ __forceinline__ float scale_of_exponent(uint32_t b) {
-  return __uint_as_float(b == 255u ? 0x7fc00000u : b == 0u ? 0x00400000u : b << 23);
-}
-template <bool E8M0>
-__device__ __forceinline__ float load_scale(const void* base, long long i) {
-  if constexpr (E8M0) {
-    uint32_t b;
-    asm volatile("ld.global.u8 %0, [%1];" : "=r"(b) : "l"(static_cast<const uint8_t*>(base) + i) : "memory");
-    return scale_of_exponent(b);
-  } else {
-    return ld_global_f32(static_cast<const float*>(base) + i);
+// The 8-bit scales of up to four K blocks from element i on, `left` of which exist, in the bytes of a word.
+__device__ __forceinline__ uint32_t load_exponents4(const void* base, long long i, long long step, int left, bool whole) {
+  const uint8_t* p = static_cast<const uint8_t*>(base) + i;
+  uint32_t w = 0;
+  if (whole && left >= 4) {
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(w) : "l"(p) : "memory");
+    return w;
   }
-}
-
-// The scales of up to four K blocks from element i on, `left` of which exist, as they lie in memory: nothing waits for the loads
-// before the first value() (where they cannot be had at once, 8-bit ones are put together on arrival).
-template <bool E8M0>
-struct Scales4 {
-  float f[4];
-  __device__ __forceinline__ void load(const void* base, long long i, long long step, int left, bool whole) {
-    if (whole && left >= 4) {
-      asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
-                   : "l"(static_cast<const float*>(base) + i) : "memory");
-      return;
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = j < left ? ld_global_f32(static_cast<const float*>(base) + i + j * step) : 0.f;
-  }
-  // Keeps the loads' first use from being moved up to them (measured: a stall of a load's latency, 900 cycles, every four K blocks).
-  __device__ __forceinline__ void arrive() { asm volatile("" : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3])); }
-  __device__ __forceinline__ float value(int j) const { return f[j]; }
-};
-template <>
-struct Scales4<true> {
-  uint32_t w;
-  __device__ __forceinline__ void load(const void* base, long long i, long long step, int left, bool whole) {
-    const uint8_t* p = static_cast<const uint8_t*>(base) + i;
-    if (whole && left >= 4) {
-      asm volatile("ld.global.b32 %0, [%1];" : "=r"(w) : "l"(p) : "memory");
-      return;
+  for (int j = 0; j < 4; ++j)
+    if (j < left) {
+      uint32_t b;
+      asm volatile("ld.global.u8 %0, [%1];" : "=r"(b) : "l"(p + j * step) : "memory");
+      w |= b << (8 * j);
     }
-    w = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < left) {
-        uint32_t b;
-        asm volatile("ld.global.u8 %0, [%1];" : "=r"(b) : "l"(p + j * step) : "memory");
-        w |= b << (8 * j);
-      }
+  return w;
+}
+// Asynchronous copies of the 32-bit scales of up to four K blocks to 16 bytes of shared memory.
+__device__ __forceinline__ void copy_scales4(uint32_t to, const float* from, long long step, int left, bool whole) {
+  if (whole && left >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    return;
   }
-  __device__ __forceinline__ void arrive() { asm volatile("" : "+r"(w)); }
-  __device__ __forceinline__ float value(int j) const { return scale_of_exponent((w >> (8 * j)) & 0xffu); }
-};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < left) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * j), "l"(from + j * step) : "memory");
+}
 
 // The exponent e of a block's scale 2^e: the smallest with amax <= 448 * 2^e, from amax's bits (448 = 1.75 * 2^8); 0 for an
 // all-zero block, never below -126, so that the scale is a normal float.
@@ -154,6 +127,11 @@ __host__ __device__ constexpr int group_table_bytes(int experts) { return 2 * (e
 __device__ __forceinline__ float lds_f32(uint32_t addr) {   // stays where it is
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 lds_f32x4(uint32_t addr) {   // 16-byte aligned; stays where it is
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ int ld_global_int(const int* p) {

@@ -23,9 +23,9 @@ struct Fp8NarrowTraits {
   static constexpr int kW = SILU ? 2 : 1;                       // weight tiles per K block
   static constexpr int kXBytes = TOK * kFp8Block;
   static constexpr int kStageBytes = kW * kFp8TileBytes + kXBytes;
-  static constexpr int kCtas = TOK * kW <= 64 ? 2 : 1;          // per SM
-  static constexpr int kStages = kCtas == 1 ? (SILU ? 5 : 4) : SILU ? 3 : TOK == 16 ? 5 : TOK == 32 ? 4 : 3;
-  static constexpr int kTmemCols = kCtas == 2 ? 256 : 512;
+  static constexpr int kCtas = SILU && TOK == 32 ? 1 : 2;       // per SM
+  static constexpr int kStages = SILU ? (TOK == 16 ? 3 : 5) : TOK == 16 ? 5 : 4;
+  static constexpr int kTmemCols = 256;
   static constexpr int kBufs = kTmemCols / (kW * TOK) > 8 ? 8 : kTmemCols / (kW * TOK);   // accumulator buffers
   static constexpr int kRing = kStages > kBufs ? kStages : kBufs;   // "block done" barriers: see the kernel
   static constexpr int kScaleBytes = 4 * kW * 4 * TOK * 4;      // [warp][weight tile][4 K blocks][TOK] floats
@@ -42,7 +42,7 @@ struct Fp8NarrowTraits {
   }
 };
 
-template <int TOK, bool E8M0, bool SILU>
+template <int TOK, bool SILU>
 __global__ void __launch_bounds__(192, (Fp8NarrowTraits<TOK, SILU>::kCtas))
 fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Fp8Params p) {
   using T = Fp8NarrowTraits<TOK, SILU>;
@@ -200,10 +200,10 @@ fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         for (int i = 0; i < kPer; ++i) {
           const int idx = lane + 32 * i, kb = kb0 + idx / TOK, tok = idx % TOK;
           const bool on = kb < kb_end && tok < t.rows;
-          xv[i] = on ? load_scale<E8M0>(p.x_scale, static_cast<long long>(t.row0 + tok) * p.xs_row + kb * p.xs_blk) : 0.f;
+          xv[i] = on ? ld_global_f32(static_cast<const float*>(p.x_scale) + static_cast<long long>(t.row0 + tok) * p.xs_row + kb * p.xs_blk) : 0.f;
 #pragma unroll
           for (int w = 0; w < kW; ++w)
-            wv[w][i] = on ? load_scale<E8M0>(p.w_scale, ws0 + static_cast<long long>(w * p.up_block0) * p.k_blocks + kb) : 0.f;
+            wv[w][i] = on ? ld_global_f32(static_cast<const float*>(p.w_scale) + ws0 + static_cast<long long>(w * p.up_block0) * p.k_blocks + kb) : 0.f;
         }
       };
       float acc[kW][TOK];
@@ -264,6 +264,7 @@ fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         const bool live = n < p.N;
 #pragma unroll
         for (int j = 0; j < TOK; ++j) {
+          if (j >= t.rows) break;
           acc[0][j] = live ? silu_times(acc[0][j], acc[1][j]) : 0.f;
           uint32_t a = __float_as_uint(acc[0][j]) & 0x7fffffffu;      // (ordered like the values; NaN above all)
           a = __reduce_max_sync(0xffffffffu, a);
@@ -280,16 +281,17 @@ fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             const int e = bad ? 0 : fp8_block_exponent(a);
             const long long m = t.row0 + j;
             if (live) out[m * p.ld_out + n] = bad ? 0x7f : static_cast<uint8_t>(e4m3x2(acc[0][j] * pow2f(-e), 0.f) & 0xff);
-            if (feature == 0) store_scale<E8M0>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
+            if (feature == 0) store_scale<false>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
           }
         }
         named_barrier_sync(1, 128);                 // (the maxima are read before the next tile's are written)
       } else if (split > 1) {
-        const int per = TOK / split;                // rows that each CTA of the cluster owns
-        const uint32_t red_at = smem_u32(red) + static_cast<uint32_t>((rank * per) * 128 + feature) * 4;
+        // CTA r of the cluster owns rows r * per .. of the tile (per is a power of two)
+        const int shift = __ffs(TOK / split) - 1;
+        const uint32_t red_at = smem_u32(red) + static_cast<uint32_t>((rank << shift) * 128 + feature) * 4;
 #pragma unroll
         for (int j = 0; j < TOK; ++j)
-          st_dsmem_f32(map_to_cta(red_at + static_cast<uint32_t>(j % per) * 512, j / per), acc[0][j]);
+          st_dsmem_f32(map_to_cta(red_at + static_cast<uint32_t>(j & ((1 << shift) - 1)) * 512, j >> shift), acc[0][j]);
       } else if (n < p.N) {
         uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<long long>(t.row0) * p.ld_out + n;
 #pragma unroll
@@ -303,13 +305,13 @@ fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     cluster_sync_all();
     if (warp < 4 && tile0 < total && !*abort_flag) {
       const Fp8Tile t = fp8_tile_at<TOK>(tile0, groups, p);
-      const int n = t.n * 128 + warp * 32 + lane, per = TOK / split;
-      uint16_t* out = static_cast<uint16_t*>(p.out) + n;
-      for (int j = 0; j < per; ++j) {
-        const int row = rank * per + j;
-        float sum = 0.f;
-        for (int r = 0; r < split; ++r) sum += red[(r * per + j) * 128 + warp * 32 + lane];
-        if (row < t.rows && n < p.N) out[static_cast<long long>(t.row0 + row) * p.ld_out] = round_out(sum, p.out_bf16);
+      const int n = t.n * 128 + warp * 32 + lane, per = TOK / split, last = min(per, t.rows - rank * per);
+      const float* from = red + warp * 32 + lane;
+      uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<long long>(t.row0 + rank * per) * p.ld_out + n;
+      for (int j = 0; j < last; ++j) {
+        float sum = from[j * 128];
+        for (int r = 1; r < split; ++r) sum += from[(r * per + j) * 128];
+        if (n < p.N) out[j * p.ld_out] = round_out(sum, p.out_bf16);
       }
     }
   }

@@ -270,16 +270,16 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         const int n_block = SILU ? t.n : 2 * t.n;
         const int second = SILU ? p.up_block0 : (n_block + 1) * 128 < p.N ? 1 : 0;
         const long long ws0 = (t.expert * p.scale_rows + n_block) * p.k_blocks, ws1 = ws0 + second * static_cast<long long>(p.k_blocks);
-        Scales4<true> x[4], w[2];
+        uint32_t x[4], w[2];
         auto fetch = [&](int kb) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = rank * 128 + lane + 32 * i;
-            x[i].load(p.x_scale, static_cast<long long>(t.row0 + (row < t.rows ? row : 0)) * p.xs_row + kb * p.xs_blk, p.xs_blk, p.k_blocks - kb,
+            x[i] = load_exponents4(p.x_scale, static_cast<long long>(t.row0 + (row < t.rows ? row : 0)) * p.xs_row + kb * p.xs_blk, p.xs_blk, p.k_blocks - kb,
                       p.x_scale_groups);
           }
-          w[0].load(p.w_scale, ws0 + kb, 1, p.k_blocks - kb, p.w_scale_groups);
-          w[1].load(p.w_scale, ws1 + kb, 1, p.k_blocks - kb, p.w_scale_groups);
+          w[0] = load_exponents4(p.w_scale, ws0 + kb, 1, p.k_blocks - kb, p.w_scale_groups);
+          w[1] = load_exponents4(p.w_scale, ws1 + kb, 1, p.k_blocks - kb, p.w_scale_groups);
         };
         fetch(0);
         for (int g = 0; g < groups_of_four; ++g) {
@@ -287,8 +287,8 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tcgen05_fence_after_sync();
-          const uint32_t sa[4] = {x[0].w, x[1].w, x[2].w, x[3].w};
-          const uint32_t sb[8] = {w[0].w, w[0].w, w[0].w, w[0].w, w[1].w, w[1].w, w[1].w, w[1].w};
+          const uint32_t sa[4] = {x[0], x[1], x[2], x[3]};
+          const uint32_t sb[8] = {w[0], w[0], w[0], w[0], w[1], w[1], w[1], w[1]};
           tmem_st_32x4(t_lane + slot * T::kSlotCols, sa);
           tmem_st_32x8(t_lane + slot * T::kSlotCols + 4, sb);
           if (g + 1 < groups_of_four) fetch(4 * g + 4);

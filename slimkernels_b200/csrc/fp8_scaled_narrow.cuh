@@ -210,15 +210,15 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
       const long long ws0 = (t.expert * p.scale_rows + t.n) * p.k_blocks;
       // groups of four are counted from this CTA's first block, which need not lie on a multiple of four
       const bool whole_w = p.w_scale_groups && (kb_begin & 3) == 0, whole_x = p.x_scale_groups && (kb_begin & 3) == 0;
-      Scales4<true> x[T::kXCols], w[kW];
+      uint32_t x[T::kXCols], w[kW];
       auto fetch = [&](int kb) {
 #pragma unroll
         for (int i = 0; i < T::kXCols; ++i) {
           const int row = lane + 32 * i;
-          x[i].load(p.x_scale, static_cast<long long>(t.row0 + (row < t.rows ? row : 0)) * p.xs_row + kb * p.xs_blk, p.xs_blk, kb_end - kb, whole_x);
+          x[i] = load_exponents4(p.x_scale, static_cast<long long>(t.row0 + (row < t.rows ? row : 0)) * p.xs_row + kb * p.xs_blk, p.xs_blk, kb_end - kb, whole_x);
         }
 #pragma unroll
-        for (int i = 0; i < kW; ++i) w[i].load(p.w_scale, ws0 + static_cast<long long>(i * p.up_block0) * p.k_blocks + kb, 1, kb_end - kb, whole_w);
+        for (int i = 0; i < kW; ++i) w[i] = load_exponents4(p.w_scale, ws0 + static_cast<long long>(i * p.up_block0) * p.k_blocks + kb, 1, kb_end - kb, whole_w);
       };
       if (kb_begin < kb_end) fetch(kb_begin);
       for (int kb = kb_begin; kb < kb_end; kb += 4) {
@@ -229,12 +229,12 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         const uint32_t at = t_lane + slot * T::kSlotCols;
 #pragma unroll
         for (int i = 0; i < kW; ++i) {
-          const uint32_t sa[4] = {w[i].w, w[i].w, w[i].w, w[i].w};
+          const uint32_t sa[4] = {w[i], w[i], w[i], w[i]};
           tmem_st_32x4(at + 4 * i, sa);
         }
         uint32_t sb[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sb[i] = x[i < T::kXCols ? i : 0].w;
+        for (int i = 0; i < 4; ++i) sb[i] = x[i < T::kXCols ? i : 0];
         tmem_st_32x4(at + 4 * kW, sb);
         if (kb + 4 < kb_end) fetch(kb + 4);
         tmem_st_wait();
@@ -286,6 +286,7 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         float h[TOK];
 #pragma unroll
         for (int j = 0; j < TOK; ++j) {
+          if (j >= t.rows) break;                   // (groups of a few rows in a tile of 32: a third of the kernel)
           h[j] = live ? silu_times(sum(0, j), sum(1, j)) : 0.f;
           uint32_t a = __float_as_uint(h[j]) & 0x7fffffffu;      // (ordered like the values; NaN above all)
           a = __reduce_max_sync(0xffffffffu, a);
@@ -307,11 +308,12 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         }
         named_barrier_sync(1, 128);                 // (the maxima are read before the next tile's are written)
       } else if (split > 1) {
-        const int per = TOK / split;                // rows that each CTA of the cluster owns
-        const uint32_t red_at = smem_u32(red) + static_cast<uint32_t>((rank * per) * 128 + feature) * 4;
+        // CTA r of the cluster owns rows r * per .. of the tile (per is a power of two)
+        const int shift = __ffs(TOK / split) - 1;
+        const uint32_t red_at = smem_u32(red) + static_cast<uint32_t>((rank << shift) * 128 + feature) * 4;
 #pragma unroll
         for (int j = 0; j < TOK; ++j)
-          st_dsmem_f32(map_to_cta(red_at + static_cast<uint32_t>(j % per) * 512, j / per), sum(0, j));
+          st_dsmem_f32(map_to_cta(red_at + static_cast<uint32_t>(j & ((1 << shift) - 1)) * 512, j >> shift), sum(0, j));
       } else if (n < p.N) {
         uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<long long>(t.row0) * p.ld_out + n;
 #pragma unroll
@@ -325,13 +327,13 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     cluster_sync_all();
     if (warp < 4 && tile0 < total && !*abort_flag) {
       const Fp8Tile t = fp8_tile_at<TOK>(tile0, groups, p);
-      const int n = t.n * 128 + warp * 32 + lane, per = TOK / split;
-      uint16_t* out = static_cast<uint16_t*>(p.out) + n;
-      for (int j = 0; j < per; ++j) {
-        const int row = rank * per + j;
-        float sum = 0.f;
-        for (int r = 0; r < split; ++r) sum += red[(r * per + j) * 128 + warp * 32 + lane];
-        if (row < t.rows && n < p.N) out[static_cast<long long>(t.row0 + row) * p.ld_out] = round_out(sum, p.out_bf16);
+      const int n = t.n * 128 + warp * 32 + lane, per = TOK / split, last = min(per, t.rows - rank * per);
+      const float* from = red + warp * 32 + lane;
+      uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<long long>(t.row0 + rank * per) * p.ld_out + n;
+      for (int j = 0; j < last; ++j) {
+        float sum = from[j * 128];
+        for (int r = 1; r < split; ++r) sum += from[(r * per + j) * 128];
+        if (n < p.N) out[j * p.ld_out] = round_out(sum, p.out_bf16);
       }
     }
   }

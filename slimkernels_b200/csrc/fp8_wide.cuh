@@ -24,8 +24,11 @@ struct Fp8WideTraits {
   static constexpr int kStageBytes = 3 * kFp8TileBytes;
   static constexpr int kOffBar = kStages * kStageBytes;
   static constexpr int kNumBars = kStages + kRing + kBufs + 1;
-  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
-  static constexpr int kOffAmax = kOffMisc + 24;    // SILU: [2 warpgroups][128 rows]
+  static constexpr int kOffMisc = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kSlots = 3;                  // groups of four K blocks whose scales are held or on their way
+  static constexpr int kOffXScale = kOffMisc + 16;  // [kSlots][256 epilogue threads][4]
+  static constexpr int kOffWScale = kOffXScale + kSlots * 256 * 16;      // [kSlots][8 warps][2 weight blocks][4]
+  static constexpr int kOffAmax = kOffWScale + kSlots * 8 * 32;          // SILU: [2 warpgroups][128 rows]
   static constexpr int kOffTable = kOffAmax + (SILU ? 2 * 128 * 4 : 0);
   static constexpr int kThreads = 384;             // two epilogue warpgroups, one for the producer and the issuer
   // Registers: 168 a thread at launch; the epilogue's 128 sums and 32 loaded values take more, the other roles less.
@@ -35,7 +38,7 @@ struct Fp8WideTraits {
 };
 static_assert(Fp8WideTraits<true>::dynamic_bytes(kFp8MaxExperts) <= 232448, "shared memory of a CTA");
 
-template <bool E8M0, bool SILU>
+template <bool SILU>
 __global__ void __launch_bounds__(384, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Fp8Params p) {
   using T = Fp8WideTraits<SILU>;
@@ -154,61 +157,80 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     int buf = 0, ring = 0;
     uint32_t done_phase = 0;
+    const uint32_t xs_slot = base + T::kOffXScale + threadIdx.x * 16, ws_slot = base + T::kOffWScale + warp * 32;
     bool ok = true;
     grid_dep_wait();
     for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
       const Fp8Tile t = fp8_tile_at<128>(tile, groups, p);
       const bool live = row < t.rows;
-      const long long xs0 = static_cast<long long>(t.row0 + (live ? row : 0)) * p.xs_row;
-      // the blocks of weight scales that this thread's columns need: one (its 128 columns), or the gate's and the up projection's
-      const int n_block = SILU ? t.n : 2 * t.n + wg;
-      const bool have = SILU || n_block * 128 < p.N;
-      const long long ws0 = (t.expert * p.scale_rows + (have ? n_block : 0)) * p.k_blocks;
-      const long long ws1 = ws0 + static_cast<long long>(SILU ? p.up_block0 : 0) * p.k_blocks;
+      // Scales come four K blocks at a time, two groups ahead, as asynchronous copies into shared memory that only this thread (a row's) or
+      // warp (the weight blocks') reads.  (As plain loads, one group ahead, they cost the epilogue a stall of 900 cycles every four K blocks,
+      // although nothing used them: a warp's few scoreboards are shared with the barriers' answers.)
+      const float* x_scale = static_cast<const float*>(p.x_scale) + static_cast<long long>(t.row0 + (live ? row : 0)) * p.xs_row;
+      // the weight blocks that this warp's columns need: one (its 128 columns; past the end any), or the gate's and the up projection's
+      const int n_block = SILU ? t.n : (2 * t.n + wg) * 128 < p.N ? 2 * t.n + wg : 2 * t.n;
+      const float* w_scale = static_cast<const float*>(p.w_scale) + (t.expert * p.scale_rows + n_block) * p.k_blocks;
+      const float* up_scale = w_scale + static_cast<long long>(p.up_block0) * p.k_blocks;
+      auto fetch = [&](int g) {                     // the scales of blocks 4 g .. 4 g + 3, as far as they exist
+        const int slot = g % T::kSlots, kb = 4 * g;
+        if (kb < p.k_blocks) {
+          copy_scales4(xs_slot + slot * (256 * 16), x_scale + kb * p.xs_blk, p.xs_blk, p.k_blocks - kb, p.x_scale_groups);
+          if (lane == 0) copy_scales4(ws_slot + slot * (8 * 32), w_scale + kb, 1, p.k_blocks - kb, p.w_scale_groups);
+          if (SILU && lane == 1) copy_scales4(ws_slot + slot * (8 * 32) + 16, up_scale + kb, 1, p.k_blocks - kb, p.w_scale_groups);
+        }
+        cp_async_commit();
+      };
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-      // scales are asked for two K blocks ahead
-      float x_next[2], w_next[2], v_next[2];
-      auto fetch = [&](int kb, int i) {
-        if (kb < p.k_blocks) {
-          x_next[i] = load_scale<E8M0>(p.x_scale, xs0 + kb * p.xs_blk);
-          w_next[i] = load_scale<E8M0>(p.w_scale, ws0 + kb);
-          if constexpr (SILU) v_next[i] = load_scale<E8M0>(p.w_scale, ws1 + kb);
-        }
-      };
-      fetch(0, 0);
-      fetch(1, 1);
-      for (int kb0 = 0; kb0 < p.k_blocks && ok; kb0 += 2) {
+      fetch(0);
+      fetch(1);
+      for (int kb0 = 0; kb0 < p.k_blocks && ok; kb0 += 4) {
+        const int slot = (kb0 >> 2) % T::kSlots;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        const float4 x4 = lds_f32x4(xs_slot + slot * (256 * 16)), w4 = lds_f32x4(ws_slot + slot * (8 * 32));
+        const float4 u4 = SILU ? lds_f32x4(ws_slot + slot * (8 * 32) + 16) : w4;
+        const float s0[4] = {x4.x * w4.x, x4.y * w4.y, x4.z * w4.z, x4.w * w4.w};
+        const float s1[4] = {x4.x * u4.x, x4.y * u4.y, x4.z * u4.z, x4.w * u4.w};
+        __syncwarp();                               // (read by all lanes before the slot is written again)
+        fetch((kb0 >> 2) + 2);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int kb = kb0 + i;
-          if (kb >= p.k_blocks) break;
-          const float s0 = x_next[i] * w_next[i];
-          const float s1 = SILU ? x_next[i] * v_next[i] : s0;
-          fetch(kb + 2, i);
+        for (int i = 0; i < 4; ++i) {
+          if (kb0 + i >= p.k_blocks) break;
           ok = wait_bounded(bar_done + 8 * ring, done_phase, ctx, kStEpilogueAccFull);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tcgen05_fence_after_sync();
+          const uint32_t from = t_lane + buf * 256 + (SILU ? wg * 64 : wg * 128);
+          uint32_t v[2][32];
+          auto load = [&](int c) { tmem_ld_32x32(from + (SILU ? (c >> 1) * 128 + (c & 1) * 32 : c * 32), v[c & 1]); };
+          auto add = [&](int c) {
+            const float f = SILU && c >= 2 ? s1[i] : s0[i];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32(t_lane + buf * 256 + (SILU ? (c >> 1) * 128 + wg * 64 + (c & 1) * 32 : wg * 128 + c * 32), v);
-            tmem_ld_wait();
-            if (c == 3) {                           // the last read of this buffer
-              tcgen05_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar_free + 8 * buf);
-            }
-            const float s = c < 2 ? s0 : s1;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(v[j]), s, acc[32 * c + j]);
-          }
+            for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(v[c & 1][j]), f, acc[32 * c + j]);
+          };
+          // 64 columns at a time: the second half's loads go out between the first half's sums, and the buffer is free again before the
+          // second half is added
+          load(0);
+          load(1);
+          tmem_ld_wait();
+          add(0);
+          load(2);
+          add(1);
+          load(3);
+          tmem_ld_wait();
+          tcgen05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_free + 8 * buf);
+          add(2);
+          add(3);
           if (++buf == B) buf = 0;
           if (++ring == R) { ring = 0; done_phase ^= 1; }
         }
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
       // (the warps of the SiLU epilogue meet below: none may be waited for that has given up)
       if constexpr (SILU) ok = named_barrier_all(1, 256, ok);
       if (!ok) break;
@@ -247,7 +269,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 if (n0 + 16 * c + j < p.N) dst[16 * c + j] = static_cast<uint8_t>(w[j >> 2] >> (8 * (j & 3)));
             }
           }
-          if (wg == 0) store_scale<E8M0>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
+          if (wg == 0) store_scale<false>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
         }
       } else if (live) {
         const int n0 = t.n * 256 + wg * 128;

@@ -96,6 +96,9 @@ bool is_float_type(int t) { return t >= SK_FLOAT_F16 && t <= SK_FLOAT_F32; }
 bool is_out_type(int t) { return t == SK_OUT_F16 || t == SK_OUT_BF16; }
 int64_t scale_bytes(int scale_type) { return scale_type == SK_SCALE_E8M0 ? 1 : 4; }
 
+// dependent: programmatic dependent launch.  Every kernel here but the weight preparation waits (griddepcontrol.wait) before it reads or
+// writes global memory, so its set-up may run under the tail of whatever is in front of it; that saves 1 to 2 us a launch between
+// this library's kernels, which let their followers start early.
 struct LaunchConfig {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -139,61 +142,79 @@ struct Choice {
   int64_t ctas;
 };
 
-// One product, or the products of a group: what decides how it is launched.
+// What a product, or the products of the groups, are launched as.  Measured on B200 (us; few rows: features on the tensor memory's lanes in tiles
+// of 16 / 32 / 64 rows, many: rows on the lanes, 128 a CTA or 256 a pair of CTAs).
+//   One group, 8-bit scales, K 4096:   64 rows x 12288   few 15.2, many 18.4, pair 18.6      256 x 4096   few 13.6, many 17.1, pair 15.3
+//                                     256 rows x 12288   few 27.3, many 20.9, pair 19.1      512 x 4096   few 16.5, many 17.0, pair 15.7
+//   so few rows' kernel takes up to 128 rows, and more for as long as its tiles of 64 rows fit the SMs at once; the pair takes the rest.
+//   One group, 32-bit scales, K 4096:  64 rows x 12288   few 19.8, many 22.9     128 x 4096   few 14.0, many 22.6     128 x 12288   few 35.7, many 25.4
+//   By expert, 16 experts x 4096 x 2048, 8-bit scales, rows per expert (ragged) 2 / 16 / 64 / 256 / 1024:
+//     few rows, tile 16  21.9 / 26.9 / 41.9     tile 32  22.6 / 26.2 / 34.2     many  27.6 / 26.9 / 28.7 / 53.3 / 148.8     pair  30.4 / 32.9 / 35.7 / 51.6 / 138.5
+//   (a pair's tiles of 256 rows are emptier at a group's end, which costs more than its faster MMAs give up to about 512 rows).
+// A tile's K range is split while that leaves an SM for every CTA and a CTA eight K blocks or so: 64 x 4096 x 4096 12.9 us in one, 10.9 in four; splitting
+// where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two).
 Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, int sms) {
   Choice c;
   const int64_t rows = ceil_div(M, experts);       // of a group, on average
-  c.kernel = rows <= 64 ? (e8m0 ? SK_FP8_KERNEL_SCALED_NARROW : SK_FP8_KERNEL_NARROW) : e8m0 ? SK_FP8_KERNEL_SCALED_PAIR : SK_FP8_KERNEL_WIDE;
-  if (const int64_t forced = g_options[SK_FP8_OPT_KERNEL].load()) c.kernel = e8m0 ? static_cast<int>(forced) : forced == SK_FP8_KERNEL_NARROW || forced == SK_FP8_KERNEL_SCALED_NARROW ? SK_FP8_KERNEL_NARROW : SK_FP8_KERNEL_WIDE;
-  const bool narrow = c.kernel == SK_FP8_KERNEL_NARROW || c.kernel == SK_FP8_KERNEL_SCALED_NARROW;
-  if (narrow) {
-    c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || silu ? 64 : 128;
-    if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(std::min<int64_t>(forced, silu ? 64 : 128));
+  const int64_t blocks = ceil_div(N, 128), kb = ceil_div(K, 128);
+  bool few;
+  if (grouped) {
+    few = rows <= 32;
+    c.row_tile = rows <= 8 ? 16 : 32;
+  } else if (e8m0) {
+    few = rows <= 128 || ceil_div(rows, 64) * blocks <= sms;
+    c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  } else {
+    few = rows <= 64 || ceil_div(rows, 32) * blocks <= sms;
+    c.row_tile = rows <= 16 ? 16 : 32;
+  }
+  c.kernel = few ? SK_FP8_KERNEL_FEW : !e8m0 || (grouped && rows <= 512) ? SK_FP8_KERNEL_MANY : SK_FP8_KERNEL_PAIR;
+  if (const int64_t forced = g_options[SK_FP8_OPT_KERNEL].load()) c.kernel = static_cast<int>(!e8m0 && forced == SK_FP8_KERNEL_PAIR ? SK_FP8_KERNEL_MANY : forced);
+  few = c.kernel == SK_FP8_KERNEL_FEW;
+  if (few) {
+    if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(forced);
+    if (silu || !e8m0) c.row_tile = std::min(c.row_tile, 32);
     c.feature_tile = 128;
   } else {
-    c.row_tile = c.kernel == SK_FP8_KERNEL_SCALED_PAIR ? 256 : 128;
+    c.row_tile = c.kernel == SK_FP8_KERNEL_PAIR ? 256 : 128;
     c.feature_tile = silu ? 128 : 256;
   }
-  const int64_t n_tiles = ceil_div(N, c.feature_tile);
-  const int64_t tiles = (grouped ? ceil_div(M, c.row_tile) + std::min(experts, M) : ceil_div(M, c.row_tile)) * n_tiles;
+  const int64_t tiles = (ceil_div(M, c.row_tile) + (grouped ? std::min(experts, M) : 0)) * ceil_div(N, c.feature_tile);
   c.split = 1;
-  if (!grouped && narrow) {
-    const int64_t kb = ceil_div(K, 128);
-    while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * 4) c.split *= 2;
+  if (!grouped && few) {
+    while (c.split < 8 && tiles * c.split * 2 <= sms && kb >= c.split * 8) c.split *= 2;
     if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
   }
   c.ctas = tiles * c.split;
   return c;
 }
 
-template <int TOK, bool E8M0, bool SILU>
-int launch_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+template <int TOK, bool SILU>
+int launch_narrow(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8NarrowTraits<TOK, SILU>;
-  auto kern = fp8_narrow_kernel<TOK, E8M0, SILU>;
-  const int smem = T::dynamic_bytes(p.split, p.experts);
+  auto kern = fp8_narrow_kernel<TOK, SILU>;
   constexpr int kMost = T::dynamic_bytes(SILU ? 1 : 8, kFp8MaxExperts);
-  static_assert(T::dynamic_bytes(SILU ? 1 : 8, 1) <= 232448 && T::dynamic_bytes(1, kFp8MaxExperts) <= 232448, "shared memory of a CTA");
+  static_assert(kMost <= 232448 && T::dynamic_bytes(SILU ? 1 : 8, 1) <= (T::kCtas == 2 ? 115712 : 232448), "shared memory of a CTA");
   // (an attribute of the function on each device; setting it again costs nothing to speak of)
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, std::min(kMost, 232448)); e != cudaSuccess)
-    return cuda_status(e);
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost); e != cudaSuccess) return cuda_status(e);
   const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * T::kCtas);
-  LaunchConfig lc(grid, 1, T::kThreads, smem, dependent, p.split, stream);
+  LaunchConfig lc(grid, 1, T::kThreads, T::dynamic_bytes(p.split, p.experts), true, p.split, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
-template <bool E8M0, bool SILU>
-int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+template <bool SILU>
+int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8WideTraits<SILU>;
-  auto kern = fp8_wide_kernel<E8M0, SILU>;
+  auto kern = fp8_wide_kernel<SILU>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::dynamic_bytes(kFp8MaxExperts)); e != cudaSuccess)
     return cuda_status(e);
-  LaunchConfig lc(std::min<int64_t>(tiles, dev.sms), 1, T::kThreads, T::dynamic_bytes(p.experts), dependent, 1, stream);
+  LaunchConfig lc(std::min<int64_t>(tiles, dev.sms), 1, T::kThreads, T::dynamic_bytes(p.experts), true, 1, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
 // The ring: 3 to 12 stages, for two CTAs per SM where there are more CTAs than SMs and two fit, else for one.
 template <int TOK, bool SILU>
-int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8ScaledNarrowTraits<TOK, SILU>;
   auto kern = fp8_scaled_narrow_kernel<TOK, SILU>;
   constexpr int kSm = 233472, kCta = 232448;        // shared memory of an SM (1 KiB per CTA goes to the system) and of a CTA
@@ -204,52 +225,40 @@ int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params
   static_assert((kCta - T::fixed_bytes(SILU ? 1 : 8, 1)) / T::kStageBytes >= 3 && (kCta - T::fixed_bytes(1, kFp8MaxExperts)) / T::kStageBytes >= 3, "room for a ring");
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kCta); e != cudaSuccess) return cuda_status(e);
   const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * ctas);
-  LaunchConfig lc(grid, 1, T::kThreads, fixed + p.stages * T::kStageBytes, dependent, p.split, stream);
+  LaunchConfig lc(grid, 1, T::kThreads, fixed + p.stages * T::kStageBytes, true, p.split, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
 template <int CTAS, bool SILU>
-int launch_scaled(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, bool dependent, cudaStream_t stream) {
+int launch_scaled(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8ScaledTraits<CTAS, SILU>;
   auto kern = fp8_scaled_kernel<CTAS, SILU>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::dynamic_bytes(kFp8MaxExperts)); e != cudaSuccess)
     return cuda_status(e);
-  LaunchConfig lc(std::min<int64_t>(tiles, dev.sms / CTAS) * CTAS, 1, T::kThreads, T::dynamic_bytes(p.experts), dependent, CTAS, stream);
+  LaunchConfig lc(std::min<int64_t>(tiles, dev.sms / CTAS) * CTAS, 1, T::kThreads, T::dynamic_bytes(p.experts), true, CTAS, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
-template <bool E8M0, bool SILU>
-int launch_product(const Choice& c, const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev,
-                   bool dependent, cudaStream_t stream) {
-  if (c.kernel == SK_FP8_KERNEL_WIDE) return launch_wide<E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-  if constexpr (E8M0) {
-    if (c.kernel == SK_FP8_KERNEL_SCALED) return launch_scaled<1, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-    if (c.kernel == SK_FP8_KERNEL_SCALED_PAIR) return launch_scaled<2, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-    if (c.kernel == SK_FP8_KERNEL_SCALED_NARROW) {
-      switch (c.row_tile) {
-        case 16: return launch_scaled_narrow<16, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-        case 32: return launch_scaled_narrow<32, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-        case 64: return launch_scaled_narrow<64, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-        default:
-          if constexpr (SILU) return SK_ERR_UNAVAILABLE;
-          else return launch_scaled_narrow<128, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-      }
-    }
+template <bool SILU>
+int launch_product(const Choice& c, bool e8m0, const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev,
+                   cudaStream_t stream) {
+  if (!e8m0) {
+    if (c.kernel == SK_FP8_KERNEL_MANY) return launch_wide<SILU>(mw, mx, p, tiles, dev, stream);
+    if (c.row_tile == 16) return launch_narrow<16, SILU>(mw, mx, p, tiles, dev, stream);
+    return launch_narrow<32, SILU>(mw, mx, p, tiles, dev, stream);
   }
-  switch (c.row_tile) {
-    case 16: return launch_narrow<16, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-    case 32: return launch_narrow<32, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-    case 64: return launch_narrow<64, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-    default:
-      if constexpr (SILU) return SK_ERR_UNAVAILABLE;
-      else return launch_narrow<128, E8M0, SILU>(mw, mx, p, tiles, dev, dependent, stream);
-  }
+  if (c.kernel == SK_FP8_KERNEL_MANY) return launch_scaled<1, SILU>(mw, mx, p, tiles, dev, stream);
+  if (c.kernel == SK_FP8_KERNEL_PAIR) return launch_scaled<2, SILU>(mw, mx, p, tiles, dev, stream);
+  if (c.row_tile == 16) return launch_scaled_narrow<16, SILU>(mw, mx, p, tiles, dev, stream);
+  if constexpr (!SILU)
+    if (c.row_tile == 64) return launch_scaled_narrow<64, SILU>(mw, mx, p, tiles, dev, stream);
+  return launch_scaled_narrow<32, SILU>(mw, mx, p, tiles, dev, stream);
 }
 
-// silu_out: the SiLU epilogue; w then holds 2 * experts matrices of N rows.  `dependent`: the previous kernel in the stream is this
-// library's and lets this one start early; early_weights: ... and no kernel that may still run wrote the weights.
+// silu_out: the SiLU epilogue; w then holds 2 * experts matrices of N rows.  early_weights: the kernel in front is this library's
+// quantiser, which starts only when the kernels that may have written the weights are complete (fp8_quantize_kernel).
 int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_type, const int32_t* offsets, void* out, int64_t ld_out,
-            int out_dtype, const sk_fp8_rows* silu_out, bool dependent, bool early_weights, cudaStream_t stream) {
+            int out_dtype, const sk_fp8_rows* silu_out, bool early_weights, cudaStream_t stream) {
   const bool silu = silu_out != nullptr;
   const int64_t experts = silu ? w->experts / 2 : w->experts;
   const int64_t N = w->N, K = w->K;
@@ -295,10 +304,8 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   CUtensorMap mw, mx;
   if (int rc = codes_map(w->q, w->experts * N, K, w->ld, 128, &mw); rc != SK_OK) return rc;
   if (int rc = codes_map(x->q, M, K, x->ld, std::min(c.row_tile, 128), &mx); rc != SK_OK) return rc;
-  return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
-    return with_bool(silu, [&](auto s) {
-      return launch_product<decltype(e8m0)::value, decltype(s)::value>(c, mw, mx, p, tiles, dev, dependent, stream);
-    });
+  return with_bool(silu, [&](auto s) {
+    return launch_product<decltype(s)::value>(c, scale_type == SK_SCALE_E8M0, mw, mx, p, tiles, dev, stream);
   });
 }
 
@@ -317,14 +324,14 @@ int check_rows(const sk_fp8_rows* x, int64_t M, int64_t K) {
 }
 
 int quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t K, const sk_fp8_rows& out, int scale_type, const int32_t* rows,
-             int64_t choices, bool dependent, cudaStream_t stream) {
+             int64_t choices, cudaStream_t stream) {
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
   const int64_t units = M * ceil_div(K, 128);
   const int64_t grid = std::min<int64_t>(ceil_div(units, 16), static_cast<int64_t>(dev.sms) * 8);
   const int64_t size = x_type == SK_FLOAT_F32 ? 4 : 2;
   const bool vector = aligned(x, 16) && ld_x * size % 16 == 0;
-  LaunchConfig lc(grid, 1, 256, 0, dependent, 1, stream);
+  LaunchConfig lc(grid, 1, 256, 0, true, 1, stream);
   return with_type(x_type, [&](auto type) {
     return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
       return with_bool(vector, [&](auto v) {
@@ -361,7 +368,7 @@ int64_t route_per_cta(int64_t T, int sms) {
 }
 
 template <int TYPE, bool TOPK>
-int launch_route(RouteParams p, int64_t ctas, bool dependent, cudaStream_t stream) {
+int launch_route(RouteParams p, int64_t ctas, cudaStream_t stream) {
   const int smem = route_smem_bytes(p.E);
   const auto go = [&](auto per) -> int {
     constexpr int kPer = decltype(per)::value;
@@ -370,7 +377,7 @@ int launch_route(RouteParams p, int64_t ctas, bool dependent, cudaStream_t strea
     auto kern = ctas == 1 ? one : many;
     if (smem > 48 * 1024)
       if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_status(e);
-    LaunchConfig lc(ctas, 1, kRouteWarps * 32, smem, dependent, 1, stream);
+    LaunchConfig lc(ctas, 1, kRouteWarps * 32, smem, true, 1, stream);
     if (cudaError_t e = cudaLaunchKernelEx(&lc.cfg, kern, p); e != cudaSuccess) return cuda_status(e);
     if (ctas == 1) return SK_OK;
     if (smem > 48 * 1024)
@@ -406,8 +413,8 @@ int route(RouteParams p, int logits_type, bool topk, int64_t T, int64_t E, int64
     if (!aligned(workspace, 4)) return SK_ERR_BAD_ALIGNMENT;
     p.counts = static_cast<int*>(workspace);
   }
-  if (!topk) return launch_route<0, false>(p, ctas, false, stream);
-  return with_type(logits_type, [&](auto type) { return launch_route<decltype(type)::value, true>(p, ctas, false, stream); });
+  if (!topk) return launch_route<0, false>(p, ctas, stream);
+  return with_type(logits_type, [&](auto type) { return launch_route<decltype(type)::value, true>(p, ctas, stream); });
 }
 
 int check_route(int64_t T, int64_t E, int64_t k) {
@@ -429,7 +436,7 @@ int sk_fp8_quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t 
   if (int rc = check_rows(out, M, K); rc != SK_OK) return rc;
   if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2)) return SK_ERR_BAD_ALIGNMENT;
   if (M == 0) return SK_OK;
-  return quantize(x, x_type, ld_x, M, K, *out, scale_type, nullptr, 1, false, static_cast<cudaStream_t>(stream));
+  return quantize(x, x_type, ld_x, M, K, *out, scale_type, nullptr, 1, static_cast<cudaStream_t>(stream));
 }
 
 int sk_fp8_prepare_weight(const void* w, int w_type, int64_t ld_w, int64_t w_matrix, int64_t matrices, int64_t N, int64_t K, uint8_t* w_q,
@@ -467,7 +474,7 @@ int sk_fp8_gemm(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int sca
   if (int rc = check_rows(x, M, w->K); rc != SK_OK) return rc;
   if (scale_type == SK_SCALE_F32 && !aligned(x->scale, 4)) return SK_ERR_BAD_ALIGNMENT;
   if (M == 0) return SK_OK;
-  return product(M, x, w, scale_type, nullptr, out, ld_out, out_dtype, nullptr, false, false, static_cast<cudaStream_t>(stream));
+  return product(M, x, w, scale_type, nullptr, out, ld_out, out_dtype, nullptr, false, static_cast<cudaStream_t>(stream));
 }
 
 int sk_fp8_grouped_gemm(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_type, const int32_t* offsets, void* out, int64_t ld_out,
@@ -477,7 +484,7 @@ int sk_fp8_grouped_gemm(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w,
   if (!offsets) return SK_ERR_NULL_POINTER;
   if (!aligned(offsets, 4) || (scale_type == SK_SCALE_F32 && !aligned(x->scale, 4))) return SK_ERR_BAD_ALIGNMENT;
   if (M == 0) return SK_OK;
-  return product(M, x, w, scale_type, offsets, out, ld_out, out_dtype, nullptr, false, false, static_cast<cudaStream_t>(stream));
+  return product(M, x, w, scale_type, offsets, out, ld_out, out_dtype, nullptr, false, static_cast<cudaStream_t>(stream));
 }
 
 int64_t sk_fp8_linear_workspace_bytes(int64_t M, int64_t K, int scale_type) {
@@ -495,8 +502,8 @@ int sk_fp8_linear(int64_t M, const void* x, int x_type, int64_t ld_x, const sk_f
   if (M == 0) return SK_OK;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const sk_fp8_rows rows = rows_in(static_cast<uint8_t*>(workspace), M, w->K, scale_type);
-  if (int rc = quantize(x, x_type, ld_x, M, w->K, rows, scale_type, nullptr, 1, true, s); rc != SK_OK) return rc;
-  return product(M, &rows, w, scale_type, nullptr, out, ld_out, out_dtype, nullptr, true, true, s);
+  if (int rc = quantize(x, x_type, ld_x, M, w->K, rows, scale_type, nullptr, 1, s); rc != SK_OK) return rc;
+  return product(M, &rows, w, scale_type, nullptr, out, ld_out, out_dtype, nullptr, true, s);
 }
 
 int64_t sk_route_workspace_bytes(int64_t T, int64_t E) {
@@ -559,9 +566,9 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
   at += rows_bytes(R, hidden, scale_type);
   const sk_fp8_rows hr = rows_in(at, R, inter, scale_type);
   at += rows_bytes(R, inter, scale_type);
-  if (int rc = quantize(x, x_type, ld_x, T, hidden, xr, scale_type, rows, k, true, s); rc != SK_OK) return rc;
-  if (int rc = product(R, &xr, gate_up, scale_type, offsets, nullptr, 0, out_dtype, &hr, true, false, s); rc != SK_OK) return rc;
-  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, out_dtype, nullptr, true, false, s); rc != SK_OK) return rc;
+  if (int rc = quantize(x, x_type, ld_x, T, hidden, xr, scale_type, rows, k, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &xr, gate_up, scale_type, offsets, nullptr, 0, out_dtype, &hr, false, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, out_dtype, nullptr, false, s); rc != SK_OK) return rc;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
   const bool vector = hidden % 8 == 0 && ld_out % 8 == 0 && aligned(out, 16);
@@ -610,7 +617,7 @@ int sk_fp8_set_option(int key, int64_t value) {
   if (value < 0) return SK_ERR_BAD_ARGUMENT;
   switch (key) {
     case SK_FP8_OPT_ROW_TILE:
-      if (value != 0 && value != 16 && value != 32 && value != 64 && value != 128) return SK_ERR_BAD_ARGUMENT;
+      if (value != 0 && value != 16 && value != 32 && value != 64) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_SPLIT_K:
       if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return SK_ERR_BAD_ARGUMENT;
@@ -619,7 +626,7 @@ int sk_fp8_set_option(int key, int64_t value) {
       if (value != 0 && value < 1000) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_KERNEL:
-      if (value > SK_FP8_KERNEL_SCALED_NARROW) return SK_ERR_BAD_ARGUMENT;
+      if (value > SK_FP8_KERNEL_PAIR) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_TEST_SKIP_COPY:
       if (value > kIntMax) return SK_ERR_BAD_ARGUMENT;

@@ -147,7 +147,7 @@ def test_router_and_experts_refuse_bad_arguments(built_libs):
 def test_options_are_checked(built_libs):
     from slimkernels_b200 import capi
     lib = capi.load()
-    for key, value in [(1, 48), (1, -1), (2, 3), (3, 10), (0, 0), (99, 0), (5, 6)]:
+    for key, value in [(1, 48), (1, -1), (2, 3), (3, 10), (0, 0), (99, 0), (5, 4), (1, 128)]:
         assert lib.sk_fp8_set_option(key, value) == capi.SK_ERR_BAD_ARGUMENT, (key, value)
     for key in (1, 2, 3, 4, 5):
         assert lib.sk_fp8_set_option(key, 0) == capi.SK_OK

@@ -184,10 +184,8 @@ def test_expert_layers(T, E, k, hidden, inter, dtype, scales):
     assert torch.equal(y, sk.fp8_experts(x, routing, *gu, *dn))
 
 
-@pytest.mark.parametrize("kernel,row_tile", [(capi.FP8_NARROW, 16), (capi.FP8_NARROW, 32), (capi.FP8_NARROW, 64), (capi.FP8_WIDE, 0),
-                                             (capi.FP8_SCALED, 0), (capi.FP8_SCALED_PAIR, 0), (capi.FP8_SCALED_NARROW, 16),
-                                             (capi.FP8_SCALED_NARROW, 32), (capi.FP8_SCALED_NARROW, 64)])
-@pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32), (272, 144, E8M0)])
+@pytest.mark.parametrize("kernel,row_tile", [(capi.FP8_FEW, 16), (capi.FP8_FEW, 32), (capi.FP8_MANY, 0), (capi.FP8_PAIR, 0)])
+@pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32), (272, 144, E8M0), (256, 1111, F32)])
 def test_expert_layers_every_kernel(kernel, row_tile, hidden, inter, scales):
     T, E, k = 500, 5, 2
     g, gu, dn = _layers(E, hidden, inter, scales, 21)

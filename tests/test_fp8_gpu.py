@@ -158,18 +158,18 @@ def test_product_at_working_sizes(M, N, K, scales):
     _check_product(*_operands(M, N, K, scales, M + N + K), torch.bfloat16)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("row_tile", [16, 32, 64])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 2048), (130, 200, 1100), (257, 1024, 1024)])
-@pytest.mark.parametrize("kernel,scales", [(capi.FP8_NARROW, E8M0), (capi.FP8_NARROW, F32), (capi.FP8_SCALED_NARROW, E8M0)])
-def test_kernels_for_few_rows_every_tile_and_split(M, N, K, kernel, scales, row_tile, split, forced):
-    forced(row_tile, split, kernel=kernel)
+@pytest.mark.parametrize("scales", [E8M0, F32])
+def test_few_rows_every_tile_and_split(M, N, K, scales, row_tile, split, forced):
+    forced(row_tile, split, kernel=capi.FP8_FEW)
     x = _operands(M, N, K, scales, 3)
     y = _check_product(*x, torch.float16)
     assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
 
 
-KERNELS = [(capi.FP8_WIDE, F32), (capi.FP8_WIDE, E8M0), (capi.FP8_SCALED, E8M0), (capi.FP8_SCALED_PAIR, E8M0), (capi.FP8_SCALED_NARROW, E8M0)]
+KERNELS = [(k, s) for k in (capi.FP8_FEW, capi.FP8_MANY, capi.FP8_PAIR) for s in (E8M0, F32) if (k, s) != (capi.FP8_PAIR, F32)]
 
 
 @pytest.mark.parametrize("kernel,scales", KERNELS)
@@ -182,12 +182,10 @@ def test_every_kernel(M, N, K, kernel, scales, forced):
     assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
 
 
-@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
-@pytest.mark.parametrize("kernel", [capi.FP8_SCALED, capi.FP8_SCALED_PAIR, capi.FP8_SCALED_NARROW])
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64])
+@pytest.mark.parametrize("kernel", [capi.FP8_FEW, capi.FP8_MANY, capi.FP8_PAIR])
 def test_every_scale_reaches_its_row_and_block(kernel, row_tile, forced):
     """Scales that differ from row to row and block to block by large factors, in any memory order: none may be taken for another's."""
-    if row_tile and kernel != capi.FP8_SCALED_NARROW:
-        pytest.skip("the row tile is the narrow kernel's")
     forced(row_tile, kernel=kernel)
     M, N, K = 300, 700, 1500
     x_q, x_s, w_q, w_s = _operands(M, N, K, E8M0, 4)
@@ -240,7 +238,7 @@ def test_nan_stays_in_its_row_and_feature(M, kernel, scales, forced):
     assert not bool(nan.any())
 
 
-@pytest.mark.parametrize("kernel", [0, capi.FP8_NARROW, capi.FP8_WIDE, capi.FP8_SCALED, capi.FP8_SCALED_PAIR])
+@pytest.mark.parametrize("kernel", [0, capi.FP8_FEW, capi.FP8_MANY, capi.FP8_PAIR])
 def test_scales_at_the_ends_of_their_range(kernel, forced):
     """2^-127 (the smallest 8-bit scale, a subnormal float) times large ones; a NaN scale; sums that leave the range of fp32.
 
@@ -339,11 +337,11 @@ def test_grouped_product(offsets, N, K, scales, out_dtype):
     _check_grouped(offsets, offsets[-1] + 9, N, K, scales, out_dtype)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64, 128])
-@pytest.mark.parametrize("kernel", [capi.FP8_NARROW, capi.FP8_SCALED_NARROW])
-def test_grouped_product_every_narrow_tile(kernel, row_tile, forced):
-    forced(row_tile, kernel=kernel)
-    _check_grouped([0, 130, 130, 131, 300, 420, 433], 440, 384, 400, E8M0, torch.float16)
+@pytest.mark.parametrize("row_tile", [16, 32, 64])
+@pytest.mark.parametrize("scales", [E8M0, F32])
+def test_grouped_product_of_few_rows_every_tile(scales, row_tile, forced):
+    forced(row_tile, kernel=capi.FP8_FEW)
+    _check_grouped([0, 130, 130, 131, 300, 420, 433], 440, 384, 400, scales, torch.float16)
 
 
 @pytest.mark.parametrize("kernel,scales", KERNELS)
@@ -455,9 +453,10 @@ def test_weights_written_on_the_way_are_seen():
     assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
 
 
-@pytest.mark.parametrize("M,kernel", [(4, 0), (4, capi.FP8_NARROW), (200, capi.FP8_NARROW), (200, capi.FP8_SCALED_NARROW), (200, capi.FP8_WIDE), (200, capi.FP8_SCALED), (500, capi.FP8_SCALED_PAIR)])
-def test_a_copy_that_never_lands_ends_in_a_status(M, kernel, forced):
-    x = _operands(M, 256, 1024, E8M0, 3)
+@pytest.mark.parametrize("M,kernel,scales", [(4, 0, E8M0), (4, 0, F32), (200, capi.FP8_FEW, E8M0), (200, capi.FP8_FEW, F32), (200, capi.FP8_MANY, E8M0),
+                                             (200, capi.FP8_MANY, F32), (500, capi.FP8_PAIR, E8M0)])
+def test_a_copy_that_never_lands_ends_in_a_status(M, kernel, scales, forced):
+    x = _operands(M, 256, 1024, scales, 3)
     forced(kernel=kernel)
     want = sk.fp8_gemm(*x)
     forced(limit=2_000_000, skip=3, kernel=kernel)
