@@ -70,7 +70,7 @@ int sk_fp8_grouped_gemm(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w,
  * the k chosen.  rows[t, j] is the place of choice (t, j) in the order of the experts and, within an expert, of t * k + j; offsets
  * [E + 1] the experts' first places.  -infinity masks an expert (it is chosen last, with weight zero; a token with nothing else
  * gets weights of zero); NaN and +infinity give the token NaN weights.  logits [T, E], row pitch ld, sk_float_type.  E <= 1024,
- * k <= min(E, 32).  workspace: sk_route_workspace_bytes(T, E) bytes of device memory. */
+ * k <= min(E, 32).  workspace: sk_route_workspace_bytes(T, E) bytes of device memory (0: none). */
 int64_t sk_route_workspace_bytes(int64_t T, int64_t E);
 int sk_route_tokens(const void* logits, int logits_type, int64_t ld, int64_t T, int64_t E, int64_t k, int renormalize, int32_t* ids,
                     float* weights, int32_t* rows, int32_t* offsets, void* workspace, int64_t workspace_bytes, sk_stream_t stream);

@@ -195,8 +195,9 @@ fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const flo
 // of a stable sort by expert and the same in every run.
 //   pass 1  (TOPK: the k largest logits of each token and their weights) and how many choices each expert got from this CTA
 //   pass 2  (after pass 1 of all CTAs) the experts' first rows, and the place of each choice
-// With one CTA both are one launch.
-constexpr int kRouteWarps = 16;
+// With one CTA both are one launch.  Latency bounds all of it (8192 tokens of 256 logits are 4 MB): 32 warps to a CTA, a token's logits
+// loaded while the one before it is worked on, and only the lane that held a winner looks through its logits again.
+constexpr int kRouteWarps = 32;
 struct RouteParams {
   const void* logits;                   // [T, ld]
   long long ld;
@@ -220,64 +221,99 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// One token: lane holds the logits of experts lane, lane + 32, ...  The choice of round j is the largest value left, the lowest
-// expert among equals.
+// The logits of one token: lane holds those of experts lane, lane + 32, ...
 template <int TYPE, int PER>
-__device__ __forceinline__ void choose_experts(const RouteParams& p, long long t, int lane) {
+__device__ __forceinline__ void load_logits(const RouteParams& p, long long t, int lane, float (&f)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) f[i] = lane + 32 * i < p.E ? load_element<TYPE>(p.logits, t * p.ld + lane + 32 * i) : 0.f;
+}
+
+// The choice of round j is the largest value left, the lowest expert among equals.
+template <int PER>
+__device__ __forceinline__ void choose_experts(const RouteParams& p, long long t, int lane, const float (&f)[PER]) {
   uint32_t key[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane + 32 * i;
-    key[i] = e < p.E ? ordered_bits(load_element<TYPE>(p.logits, t * p.ld + e)) : 0u;   // (0 is below -infinity's bits)
-  }
-  float top = 0.f, sum = 0.f, mine = 0.f;
-  uint32_t first_bits = 0;
-  if (!p.renormalize) {
-    uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) best = max(best, key[i]);
-    first_bits = __reduce_max_sync(0xffffffffu, best);
-    top = from_ordered_bits(first_bits);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i < p.E) sum += expf(from_ordered_bits(key[i]) - top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  }
-  for (int j = 0; j < p.k; ++j) {
-    uint32_t best = 0;
-    int at = 0x7fffffff;
+  for (int i = 0; i < PER; ++i) key[i] = lane + 32 * i < p.E ? ordered_bits(f[i]) : 0u;      // (0 is below -infinity's bits)
+  uint32_t best = 0;
+  int at = 0;
+  auto look = [&]() {                   // the lane's own largest; 0: none left
+    best = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+  };
+  look();
+  float top = 0.f, sum = 0.f, mine = 0.f;
+  uint32_t first_bits = 0;
+  int my_id = 0;
+  for (int j = 0; j < p.k; ++j) {
     const uint32_t winner = __reduce_max_sync(0xffffffffu, best);
-    const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
+    const uint32_t holders = __ballot_sync(0xffffffffu, best == winner);
+    int e = __shfl_sync(0xffffffffu, at, __ffs(holders) - 1);
+    if (holders & (holders - 1)) e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
+    if (j == 0) {
+      first_bits = winner;
+      top = from_ordered_bits(winner);
+      if (!p.renormalize) {             // the whole softmax's sum, while all keys are there
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i == e) key[i] = 0;
-    if (j == 0) { first_bits = winner; top = from_ordered_bits(winner); }
+        for (int i = 0; i < PER; ++i)
+          if (lane + 32 * i < p.E) sum += expf(from_ordered_bits(key[i]) - top);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+    }
+    if ((e & 31) == lane) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (lane + 32 * i == e) key[i] = 0;
+      look();
+    }
     const float w = expf(from_ordered_bits(winner) - top);
     if (p.renormalize) sum += w;
-    if (lane == j) mine = w;
-    if (lane == 0) p.ids[t * p.k + j] = e;
+    if (lane == j) { mine = w; my_id = e; }
   }
-  // a token whose logits are all -infinity has no distribution: its weights are zero
-  if (lane < p.k) p.weights[t * p.k + lane] = first_bits == 0x007fffffu ? 0.f : mine / sum;
+  if (lane < p.k) {
+    p.ids[t * p.k + lane] = my_id;
+    // a token whose logits are all -infinity has no distribution: its weights are zero
+    p.weights[t * p.k + lane] = first_bits == 0x007fffffu ? 0.f : mine / sum;
+  }
 }
 
-template <int TYPE, int PER, bool TOPK>
-__device__ __forceinline__ void route_count(const RouteParams& p, int* hist /* [kRouteWarps][E] */) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kRouteWarps * p.E; i += kRouteWarps * 32) hist[i] = 0;
-  __syncthreads();
+struct RouteRange { long long t0, t1; };   // tokens of this warp
+__device__ __forceinline__ RouteRange route_range(const RouteParams& p) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
   const long long c0 = static_cast<long long>(blockIdx.x) * p.per_cta, c1 = min(static_cast<long long>(p.T), c0 + p.per_cta);
-  const int per_warp = (p.per_cta + kRouteWarps - 1) / kRouteWarps;
-  const long long t0 = min(c1, c0 + static_cast<long long>(warp) * per_warp), t1 = min(c1, t0 + per_warp);
+  const int per_warp = (p.per_cta + warps - 1) / warps;
+  RouteRange r;
+  r.t0 = min(c1, c0 + static_cast<long long>(warp) * per_warp);
+  r.t1 = min(c1, r.t0 + per_warp);
+  return r;
+}
+
+// hist [warps][E]: how many choices each expert got from each warp.
+template <int TYPE, int PER, bool TOPK>
+__device__ __forceinline__ void route_count(const RouteParams& p, int* hist) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const RouteRange r = route_range(p);
   if constexpr (TOPK) {
-    for (long long t = t0; t < t1; ++t) choose_experts<TYPE, PER>(p, t, lane);
+    float f[PER];
+    if (r.t0 < r.t1) load_logits<TYPE, PER>(p, r.t0, lane, f);
+    for (int i = threadIdx.x; i < warps * p.E; i += blockDim.x) hist[i] = 0;
+    for (long long t = r.t0; t < r.t1; ++t) {
+      float next[PER];
+      if (t + 1 < r.t1) load_logits<TYPE, PER>(p, t + 1, lane, next);
+      choose_experts<PER>(p, t, lane, f);
+      if (t + 1 < r.t1) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) f[i] = next[i];
+      }
+    }
     __syncwarp();
+  } else {
+    for (int i = threadIdx.x; i < warps * p.E; i += blockDim.x) hist[i] = 0;
   }
-  for (long long i = t0 * p.k + lane; i < t1 * p.k; i += 32) {
+  __syncthreads();
+  for (long long i = r.t0 * p.k + lane; i < r.t1 * p.k; i += 32) {
     const int e = p.ids[i];
     if (e >= 0 && e < p.E) atomicAdd(hist + warp * p.E + e, 1);      // (integers: the order does not show)
   }
@@ -286,23 +322,21 @@ __device__ __forceinline__ void route_count(const RouteParams& p, int* hist /* [
 
 // hist: on entry the warps' counts, on return each warp's next place for every expert.  base: the experts' first places of this CTA.
 __device__ __forceinline__ void route_place(const RouteParams& p, int* hist, const int* base) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int at = base[e];
-    for (int w = 0; w < kRouteWarps; ++w) {
+    for (int w = 0; w < warps; ++w) {
       const int n = hist[w * p.E + e];
       hist[w * p.E + e] = at;
       at += n;
     }
   }
   __syncthreads();
-  const long long c0 = static_cast<long long>(blockIdx.x) * p.per_cta, c1 = min(static_cast<long long>(p.T), c0 + p.per_cta);
-  const int per_warp = (p.per_cta + kRouteWarps - 1) / kRouteWarps;
-  const long long t0 = min(c1, c0 + static_cast<long long>(warp) * per_warp), t1 = min(c1, t0 + per_warp);
+  const RouteRange r = route_range(p);
   int* next = hist + warp * p.E;
-  for (long long i0 = t0 * p.k; i0 < t1 * p.k; i0 += 32) {
+  for (long long i0 = r.t0 * p.k; i0 < r.t1 * p.k; i0 += 32) {
     const long long i = i0 + lane;
-    const int e = i < t1 * p.k ? p.ids[i] : -1;
+    const int e = i < r.t1 * p.k ? p.ids[i] : -1;
     const bool on = e >= 0 && e < p.E;
     const uint32_t same = __match_any_sync(0xffffffffu, on ? e : -1);
     const int before = __popc(same & ((1u << lane) - 1u));
@@ -310,7 +344,7 @@ __device__ __forceinline__ void route_place(const RouteParams& p, int* hist, con
     __syncwarp();
     if (on && before == 0) next[e] += __popc(same);
     __syncwarp();
-    if (i < t1 * p.k) p.rows[i] = at;
+    if (i < r.t1 * p.k) p.rows[i] = at;
   }
 }
 
@@ -335,27 +369,28 @@ __device__ __forceinline__ void scan_experts(int* total, int E) {
   __syncthreads();
 }
 
-// Shared memory: [kRouteWarps][E] counts, [E + 1] totals, [E] first places of this CTA.
-__host__ __device__ constexpr int route_smem_bytes(int E) { return (kRouteWarps * E + 2 * E + 1) * 4; }
+// Shared memory: [warps][E] counts, [E + 1] totals, [E] first places of this CTA.
+__host__ __device__ constexpr int route_smem_bytes(int warps, int E) { return (warps * E + 2 * E + 1) * 4; }
 
 template <int TYPE, int PER, bool TOPK, bool ONE_CTA>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_count_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
+  const int warps = blockDim.x >> 5;
   int* hist = route_smem;
-  int* total = hist + kRouteWarps * p.E;
+  int* total = hist + warps * p.E;
   grid_dep_wait();
   grid_dep_launch_dependents();
   route_count<TYPE, PER, TOPK>(p, hist);
-  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) {
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int n = 0;
-    for (int w = 0; w < kRouteWarps; ++w) n += hist[w * p.E + e];
+    for (int w = 0; w < warps; ++w) n += hist[w * p.E + e];
     if constexpr (ONE_CTA) total[e] = n; else p.counts[static_cast<long long>(blockIdx.x) * p.E + e] = n;
   }
   if constexpr (ONE_CTA) {
     __syncthreads();
     scan_experts(total, p.E);
-    for (int e = threadIdx.x; e <= p.E; e += kRouteWarps * 32) p.offsets[e] = total[e];
+    for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = total[e];
     route_place(p, hist, total);
   }
 }
@@ -363,27 +398,33 @@ route_count_kernel(const RouteParams p) {
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_place_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
+  const int warps = blockDim.x >> 5;
   int* hist = route_smem;
-  int* total = hist + kRouteWarps * p.E;
+  int* total = hist + warps * p.E;
   int* base = total + p.E + 1;
   grid_dep_wait();
   grid_dep_launch_dependents();
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) total[e] = base[e] = 0;
   route_count<0, 1, false>(p, hist);                 // this CTA's counts by warp, again
-  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) {
+  // the counts of all CTAs, and of those in front of this one: as many threads per expert as there are
+  const int share = max(1, static_cast<int>(blockDim.x) / p.E), ctas = static_cast<int>(gridDim.x);
+  for (int i = threadIdx.x; i < share * p.E; i += blockDim.x) {
+    const int e = i % p.E, part = i / p.E;
     int before = 0, all = 0;
-    for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
-      const int n = ld_global_int(p.counts + static_cast<long long>(c) * p.E + e);
-      if (c < static_cast<int>(blockIdx.x)) before += n;
+#pragma unroll 16
+    for (int c = part; c < ctas; c += share) {
+      const int n = p.counts[static_cast<long long>(c) * p.E + e];
+      before += c < static_cast<int>(blockIdx.x) ? n : 0;
       all += n;
     }
-    total[e] = all;
-    base[e] = before;
+    atomicAdd(total + e, all);
+    atomicAdd(base + e, before);
   }
   __syncthreads();
   scan_experts(total, p.E);
-  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) base[e] += total[e];
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) base[e] += total[e];
   if (blockIdx.x == 0)
-    for (int e = threadIdx.x; e <= p.E; e += kRouteWarps * 32) p.offsets[e] = total[e];
+    for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = total[e];
   __syncthreads();
   route_place(p, hist, base);
 }

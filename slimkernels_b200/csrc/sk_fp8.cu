@@ -344,46 +344,43 @@ int quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t K, cons
   });
 }
 
-// Codes and scales of [M, K] in a workspace.  8-bit scales lie row by row, 32-bit ones block by block: that is how the
-// products read them, a row's four blocks at once or 32 rows of a block at once.
+// Codes and scales of [M, K] in a workspace.  The scales lie row by row, rows padded to four: the products read four K blocks' at once.
+int64_t scale_pitch(int64_t K) { return round_up(ceil_div(K, 128), 4); }
 int64_t rows_bytes(int64_t M, int64_t K, int scale_type) {
-  return round_up(M * round_up(K, 16), 256) + round_up(M * ceil_div(K, 128) * scale_bytes(scale_type), 256);
+  return round_up(M * round_up(K, 16), 256) + round_up(M * scale_pitch(K) * scale_bytes(scale_type), 256);
 }
 sk_fp8_rows rows_in(uint8_t* at, int64_t M, int64_t K, int scale_type) {
-  const int64_t kb = ceil_div(K, 128), ld = round_up(K, 16);
   sk_fp8_rows r;
   r.q = at;
-  r.ld = ld;
-  r.scale = at + round_up(M * ld, 256);
-  r.scale_row = scale_type == SK_SCALE_E8M0 ? kb : 1;
-  r.scale_block = scale_type == SK_SCALE_E8M0 ? 1 : M;
+  r.ld = round_up(K, 16);
+  r.scale = at + round_up(M * r.ld, 256);
+  r.scale_row = scale_pitch(K);
+  r.scale_block = 1;
   return r;
 }
 
 // ---------------------------------------------------------------- router
-// Tokens per CTA: one CTA for as long as its warps have a token or two each, then enough for one CTA per SM.
+// Tokens per CTA: one CTA for as long as its warps have two tokens each, then enough for one CTA per SM.
 int64_t route_per_cta(int64_t T, int sms) {
-  if (T <= 4 * kRouteWarps) return std::max<int64_t>(T, 1);
-  return std::max<int64_t>(2 * kRouteWarps, round_up(ceil_div(T, sms), kRouteWarps));
+  if (T <= 2 * kRouteWarps) return std::max<int64_t>(T, 1);
+  return std::max<int64_t>(kRouteWarps, round_up(ceil_div(T, sms), kRouteWarps));
 }
 
 template <int TYPE, bool TOPK>
 int launch_route(RouteParams p, int64_t ctas, cudaStream_t stream) {
-  const int smem = route_smem_bytes(p.E);
+  // (as many warps as there is work for, four at least: the experts' sums are spread over all threads)
+  const int warps = std::min(kRouteWarps, std::max(4, TOPK ? p.per_cta : static_cast<int>(ceil_div(static_cast<int64_t>(p.per_cta) * p.k, 32))));
+  const int smem = route_smem_bytes(warps, p.E);
+  const auto allow = [&](auto kern) { return smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess; };
   const auto go = [&](auto per) -> int {
     constexpr int kPer = decltype(per)::value;
-    auto one = route_count_kernel<TYPE, kPer, TOPK, true>;
-    auto many = route_count_kernel<TYPE, kPer, TOPK, false>;
-    auto kern = ctas == 1 ? one : many;
-    if (smem > 48 * 1024)
-      if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_status(e);
-    LaunchConfig lc(ctas, 1, kRouteWarps * 32, smem, true, 1, stream);
+    auto kern = ctas == 1 ? route_count_kernel<TYPE, kPer, TOPK, true> : route_count_kernel<TYPE, kPer, TOPK, false>;
+    if (cudaError_t e = allow(kern); e != cudaSuccess) return cuda_status(e);
+    LaunchConfig lc(ctas, 1, warps * 32, smem, true, 1, stream);
     if (cudaError_t e = cudaLaunchKernelEx(&lc.cfg, kern, p); e != cudaSuccess) return cuda_status(e);
     if (ctas == 1) return SK_OK;
-    if (smem > 48 * 1024)
-      if (cudaError_t e = cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess)
-        return cuda_status(e);
-    LaunchConfig second(ctas, 1, kRouteWarps * 32, smem, true, 1, stream);
+    if (cudaError_t e = allow(route_place_kernel); e != cudaSuccess) return cuda_status(e);
+    LaunchConfig second(ctas, 1, warps * 32, smem, true, 1, stream);
     return cuda_status(cudaLaunchKernelEx(&second.cfg, route_place_kernel, p));
   };
   if constexpr (!TOPK) {
@@ -509,7 +506,7 @@ int sk_fp8_linear(int64_t M, const void* x, int x_type, int64_t ld_x, const sk_f
 int64_t sk_route_workspace_bytes(int64_t T, int64_t E) {
   if (check_route(T, E, 1) != SK_OK) return 0;
   // (never more CTAs than this, whatever the device)
-  return std::min<int64_t>(ceil_div(std::max<int64_t>(T, 1), 2 * kRouteWarps), 1024) * E * 4;
+  return T <= 2 * kRouteWarps ? 0 : std::min<int64_t>(ceil_div(T, kRouteWarps), 1024) * E * 4;
 }
 
 int sk_route_tokens(const void* logits, int logits_type, int64_t ld, int64_t T, int64_t E, int64_t k, int renormalize, int32_t* ids, float* weights,

@@ -133,7 +133,7 @@ int one_scale_type(const at::Tensor& a, const at::Tensor& b) {
 std::tuple<at::Tensor, at::Tensor> empty_rows(const at::Tensor& like, int64_t M, int64_t K, at::ScalarType scales) {
   const int64_t kb = ceil_div(K, 128);
   at::Tensor q = at::empty({M, round_up(K, 16)}, like.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, K);
-  at::Tensor s = scales == at::kFloat ? at::empty({kb, M}, like.options().dtype(scales)).t() : at::empty({M, kb}, like.options().dtype(scales));
+  at::Tensor s = at::empty({M, round_up(kb, 4)}, like.options().dtype(scales)).narrow(1, 0, kb);
   return {q, s};
 }
 
@@ -273,7 +273,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_tokens(const at
   at::Tensor ids = at::empty({T, k}, ints), weights = at::empty({T, k}, l.options().dtype(at::kFloat)), rows = at::empty({T, k}, ints);
   at::Tensor offsets = at::empty({E + 1}, ints);
   const int64_t bytes = sk_route_workspace_bytes(T, E);
-  at::Tensor ws = at::empty({bytes}, l.options().dtype(at::kByte));
+  at::Tensor ws = bytes > 0 ? at::empty({bytes}, l.options().dtype(at::kByte)) : offsets;
   // (an empty tensor has no address; nothing is read or written through these when T = 0)
   void* some = offsets.data_ptr();
   check(sk_route_tokens(T ? l.data_ptr() : some, ft, T ? pitch(l) : E, T, E, k, renormalize, static_cast<int*>(T ? ids.data_ptr() : some),
@@ -293,7 +293,7 @@ std::tuple<at::Tensor, at::Tensor> group_by_expert(const at::Tensor& ids_in, int
   const int64_t T = ids.size(0), k = ids.size(1);
   at::Tensor rows = at::empty({T, k}, ids.options()), offsets = at::empty({E + 1}, ids.options());
   const int64_t bytes = sk_route_workspace_bytes(T, E);
-  at::Tensor ws = at::empty({bytes}, ids.options().dtype(at::kByte));
+  at::Tensor ws = bytes > 0 ? at::empty({bytes}, ids.options().dtype(at::kByte)) : offsets;
   void* some = offsets.data_ptr();
   check(sk_group_by_expert(static_cast<const int*>(T ? ids.data_ptr() : some), T, k, E, static_cast<int*>(T ? rows.data_ptr() : some),
                            offsets.data_ptr<int>(), ws.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()),

@@ -16,6 +16,17 @@ from torch import nn
 
 from .ops import load_extension
 
+_ops = {}
+
+
+def _op(name):
+    """The registered op (its only overload: looking that up on every call takes 2 us)."""
+    op = _ops.get(name)
+    if op is None:
+        load_extension()
+        op = _ops[name] = getattr(torch.ops.slimkernels, name).default
+    return op
+
 
 def quantize_fp8(x, scale_dtype=torch.float8_e8m0fnu):
     """x [..., K] (float16 / bfloat16 / float32) -> (codes [..., K], scales [..., ceil(K / 128)]).
@@ -24,31 +35,27 @@ def quantize_fp8(x, scale_dtype=torch.float8_e8m0fnu):
     code = x / scale rounded to nearest even.  A block with an infinity or a NaN becomes NaN.  The rows of the codes start on 16
     bytes, as the products want them.
     """
-    load_extension()
-    return torch.ops.slimkernels.quantize_fp8(x, scale_dtype)
+    return _op("quantize_fp8")(x, scale_dtype)
 
 
 def prepare_weight_fp8(w, scale_dtype=torch.float8_e8m0fnu):
     """w [..., N, K] -> (codes [..., N, K], scales [..., ceil(N / 128), ceil(K / 128)]), by the same rule per 128 x 128 block."""
-    load_extension()
-    return torch.ops.slimkernels.prepare_weight_fp8(w.detach(), scale_dtype)
+    return _op("prepare_weight_fp8")(w.detach(), scale_dtype)
 
 
 def fp8_gemm(x_q, x_scale, w_q, w_scale, out_dtype=torch.bfloat16, out=None):
     """[M, N] = (x_q * x_scale) @ (w_q * w_scale).T, summed in fp32 (a sum over blocks that
     leaves its range is not finite) and rounded once.  `out` may be a column slice."""
-    load_extension()
     if out is None:
-        return torch.ops.slimkernels.fp8_gemm(x_q, x_scale, w_q, w_scale, out_dtype)
-    torch.ops.slimkernels.fp8_gemm_out(x_q, x_scale, w_q, w_scale, out)
+        return _op("fp8_gemm")(x_q, x_scale, w_q, w_scale, out_dtype)
+    _op("fp8_gemm_out")(x_q, x_scale, w_q, w_scale, out)
     return out
 
 
 def fp8_linear(x, w_q, w_scale, out_dtype=None):
     """x [..., K] -> [..., N]: `quantize_fp8` with the weight's type of scales, then `fp8_gemm`.  The result has x's type where that
     has 16 bits, else float16."""
-    load_extension()
-    return torch.ops.slimkernels.fp8_linear(x, w_q, w_scale, out_dtype)
+    return _op("fp8_linear")(x, w_q, w_scale, out_dtype)
 
 
 def fp8_grouped_gemm(x_q, x_scale, w_q, w_scale, offsets, out_dtype=torch.bfloat16, out=None):
@@ -57,10 +64,9 @@ def fp8_grouped_gemm(x_q, x_scale, w_q, w_scale, offsets, out_dtype=torch.bfloat
     Groups may be empty.  Rows that belong to no group are not written: in a given `out` they keep what they held, in a fresh
     result they hold anything.
     """
-    load_extension()
     if out is None:
-        return torch.ops.slimkernels.fp8_grouped_gemm(x_q, x_scale, w_q, w_scale, offsets, out_dtype)
-    torch.ops.slimkernels.fp8_grouped_gemm_out(x_q, x_scale, w_q, w_scale, offsets, out)
+        return _op("fp8_grouped_gemm")(x_q, x_scale, w_q, w_scale, offsets, out_dtype)
+    _op("fp8_grouped_gemm_out")(x_q, x_scale, w_q, w_scale, offsets, out)
     return out
 
 
@@ -78,14 +84,12 @@ def route_tokens(logits, k, renormalize=True) -> Routing:
     -infinity masks an expert: it is chosen after all others and has weight zero; a token with nothing else gets weights of zero.
     NaN or +infinity gives the token NaN weights.  E <= 1024, k <= min(E, 32).
     """
-    load_extension()
-    return Routing(*torch.ops.slimkernels.route_tokens(logits, k, renormalize))
+    return Routing(*_op("route_tokens")(logits, k, renormalize))
 
 
 def group_by_expert(expert_ids, experts: int):
     """(rows, offsets) of a `Routing` for experts [T, k] chosen elsewhere.  Ids outside [0, experts) are nobody's: their rows are -1."""
-    load_extension()
-    return torch.ops.slimkernels.group_by_expert(expert_ids, experts)
+    return _op("group_by_expert")(expert_ids, experts)
 
 
 def fp8_experts(x, routing: Routing, gate_up, gate_up_scale, down, down_scale, out_dtype=None):
@@ -95,15 +99,13 @@ def fp8_experts(x, routing: Routing, gate_up, gate_up_scale, down, down_scale, o
     kernels: quantise into the groups' rows, grouped product with SiLU * up and the re-quantisation in its epilogue, grouped
     product, weighted sum.
     """
-    load_extension()
-    return torch.ops.slimkernels.fp8_experts(x, routing.rows, routing.weights, routing.offsets, gate_up, gate_up_scale, down, down_scale, out_dtype)
+    return _op("fp8_experts")(x, routing.rows, routing.weights, routing.offsets, gate_up, gate_up_scale, down, down_scale, out_dtype)
 
 
 def fp8_device_status(device=None) -> int:
     """Reads and clears the device's note of a wait inside an FP8 kernel that ran into its limit (0: none).  Synchronises."""
-    load_extension()
     index = torch.cuda.current_device() if device is None else torch.device(device).index
-    return torch.ops.slimkernels.fp8_device_status(torch.cuda.current_device() if index is None else index)
+    return _op("fp8_device_status")(torch.cuda.current_device() if index is None else index)
 
 
 def _padded_codes(w, scale_dtype):
