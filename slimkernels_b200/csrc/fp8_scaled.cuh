@@ -161,7 +161,7 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     }
   }
   if (p.offsets != nullptr && warp == 0) {
-    grid_dep_wait();
+    if (!p.early_weights) grid_dep_wait();
     build_group_table<kRows>(groups, p, lane);
   }
   tcgen05_fence_before_sync();

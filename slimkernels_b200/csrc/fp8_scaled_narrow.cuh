@@ -94,7 +94,7 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     tmem_relinquish();
   }
   if (p.offsets != nullptr && warp == 0) {
-    grid_dep_wait();
+    if (!p.early_weights) grid_dep_wait();
     build_group_table<TOK>(groups, p, lane);
   }
   tcgen05_fence_before_sync();
@@ -113,15 +113,15 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
       int stage = 0, early = 0, issued = 0;          // (issued counts up to `early` only)
       uint32_t phase = 1;                           // (the first round of stages is free)
       bool ok = true;
-      if (p.early_weights && tile0 < total) {       // (one group of rows, weights that no kernel still in flight writes)
+      if (p.early_weights && tile0 < total) {       // (weights that no kernel still in flight writes)
         const Fp8Tile t = fp8_tile_at<TOK>(tile0, groups, p);
         early = min(S, kb_end - kb_begin);
         for (int i = 0; i < early; ++i) {
           if (kb_begin + i == p.skip_block) continue;
           mbar_arrive_expect_tx(bar_full + 8 * i, T::kStageBytes);
           for (int w = 0; w < kW; ++w)
-            tma_load_2d(base + i * T::kStageBytes + w * kFp8TileBytes, &tmap_w, (kb_begin + i) * kFp8Block, t.n * 128 + w * p.up_row0,
-                        bar_full + 8 * i);
+            tma_load_2d(base + i * T::kStageBytes + w * kFp8TileBytes, &tmap_w, (kb_begin + i) * kFp8Block,
+                        t.expert * p.w_rows + t.n * 128 + w * p.up_row0, bar_full + 8 * i);
         }
       }
       grid_dep_wait();

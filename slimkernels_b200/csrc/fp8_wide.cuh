@@ -70,7 +70,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     tmem_relinquish();
   }
   if (p.offsets != nullptr && warp == 0) {
-    grid_dep_wait();
+    if (!p.early_weights) grid_dep_wait();
     build_group_table<128>(groups, p, lane);
   }
   tcgen05_fence_before_sync();

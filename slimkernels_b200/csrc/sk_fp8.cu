@@ -28,6 +28,7 @@ int cuda_status(cudaError_t e) {
 }
 
 struct DeviceInfo {
+  int index = 0;
   int sms = 0;
   int* status = nullptr;
 };
@@ -55,6 +56,7 @@ int device_info(DeviceInfo* out) {
     words[dev].store(static_cast<int*>(word));
     sms[dev].store(n);
   }
+  out->index = dev;
   out->sms = sms[dev].load();
   out->status = words[dev].load();
   return SK_OK;
@@ -120,6 +122,16 @@ struct LaunchConfig {
     }
   }
 };
+
+// Lets a kernel have so much shared memory: once per kernel and device (`done` belongs to the kernel).
+template <class Kernel>
+int allow_shared(Kernel kern, int bytes, const DeviceInfo& dev, std::atomic<uint64_t>& done) {
+  const uint64_t bit = uint64_t(1) << dev.index;
+  if (done.load(std::memory_order_acquire) & bit) return SK_OK;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) return cuda_status(e);
+  done.fetch_or(bit, std::memory_order_release);
+  return SK_OK;
+}
 
 // Calls fn(std::integral_constant...) for a runtime value.
 template <class F>
@@ -195,8 +207,8 @@ int launch_narrow(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params&
   auto kern = fp8_narrow_kernel<TOK, SILU>;
   constexpr int kMost = T::dynamic_bytes(SILU ? 1 : 8, kFp8MaxExperts);
   static_assert(kMost <= 232448 && T::dynamic_bytes(SILU ? 1 : 8, 1) <= (T::kCtas == 2 ? 115712 : 232448), "shared memory of a CTA");
-  // (an attribute of the function on each device; setting it again costs nothing to speak of)
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost); e != cudaSuccess) return cuda_status(e);
+  static std::atomic<uint64_t> done;
+  if (int rc = allow_shared(kern, kMost, dev, done); rc != SK_OK) return rc;
   const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * T::kCtas);
   LaunchConfig lc(grid, 1, T::kThreads, T::dynamic_bytes(p.split, p.experts), true, p.split, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
@@ -206,8 +218,8 @@ template <bool SILU>
 int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8WideTraits<SILU>;
   auto kern = fp8_wide_kernel<SILU>;
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::dynamic_bytes(kFp8MaxExperts)); e != cudaSuccess)
-    return cuda_status(e);
+  static std::atomic<uint64_t> done;
+  if (int rc = allow_shared(kern, T::dynamic_bytes(kFp8MaxExperts), dev, done); rc != SK_OK) return rc;
   LaunchConfig lc(std::min<int64_t>(tiles, dev.sms), 1, T::kThreads, T::dynamic_bytes(p.experts), true, 1, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
@@ -223,7 +235,8 @@ int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params
   if ((kSm / ctas - 1024 - fixed) / T::kStageBytes < 3) ctas = 1;
   p.stages = std::min(T::kMaxStages, ((ctas == 1 ? kCta : kSm / 2 - 1024) - fixed) / T::kStageBytes);
   static_assert((kCta - T::fixed_bytes(SILU ? 1 : 8, 1)) / T::kStageBytes >= 3 && (kCta - T::fixed_bytes(1, kFp8MaxExperts)) / T::kStageBytes >= 3, "room for a ring");
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kCta); e != cudaSuccess) return cuda_status(e);
+  static std::atomic<uint64_t> done;
+  if (int rc = allow_shared(kern, kCta, dev, done); rc != SK_OK) return rc;
   const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * ctas);
   LaunchConfig lc(grid, 1, T::kThreads, fixed + p.stages * T::kStageBytes, true, p.split, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
@@ -233,8 +246,8 @@ template <int CTAS, bool SILU>
 int launch_scaled(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8ScaledTraits<CTAS, SILU>;
   auto kern = fp8_scaled_kernel<CTAS, SILU>;
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::dynamic_bytes(kFp8MaxExperts)); e != cudaSuccess)
-    return cuda_status(e);
+  static std::atomic<uint64_t> done;
+  if (int rc = allow_shared(kern, T::dynamic_bytes(kFp8MaxExperts), dev, done); rc != SK_OK) return rc;
   LaunchConfig lc(std::min<int64_t>(tiles, dev.sms / CTAS) * CTAS, 1, T::kThreads, T::dynamic_bytes(p.experts), true, CTAS, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
@@ -255,8 +268,9 @@ int launch_product(const Choice& c, bool e8m0, const CUtensorMap& mw, const CUte
   return launch_scaled_narrow<32, SILU>(mw, mx, p, tiles, dev, stream);
 }
 
-// silu_out: the SiLU epilogue; w then holds 2 * experts matrices of N rows.  early_weights: the kernel in front is this library's
-// quantiser, which starts only when the kernels that may have written the weights are complete (fp8_quantize_kernel).
+// silu_out: the SiLU epilogue; w then holds 2 * experts matrices of N rows.  early_weights: this library's quantiser is in front, or a product
+// of the same call with it in front.  It lets its followers start only when all kernels in front of it are complete (fp8_quantize_kernel), those
+// among them that wrote the weights or the groups' offsets, so both may be read before this kernel's own wait.
 int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_type, const int32_t* offsets, void* out, int64_t ld_out,
             int out_dtype, const sk_fp8_rows* silu_out, bool early_weights, cudaStream_t stream) {
   const bool silu = silu_out != nullptr;
@@ -293,7 +307,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   const int64_t four = 4 * scale_bytes(scale_type);
   p.x_scale_groups = p.xs_blk == 1 && p.xs_row % 4 == 0 && aligned(p.x_scale, four);
   p.w_scale_groups = p.k_blocks % 4 == 0 && aligned(p.w_scale, four);
-  p.early_weights = early_weights && offsets == nullptr;
+  p.early_weights = early_weights;
   p.split = c.split;
   p.skip_block = static_cast<int>(g_options[SK_FP8_OPT_TEST_SKIP_COPY].load()) - 1;
   const int64_t limit = g_options[SK_FP8_OPT_WAIT_LIMIT_CYCLES].load();
@@ -564,8 +578,8 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
   const sk_fp8_rows hr = rows_in(at, R, inter, scale_type);
   at += rows_bytes(R, inter, scale_type);
   if (int rc = quantize(x, x_type, ld_x, T, hidden, xr, scale_type, rows, k, s); rc != SK_OK) return rc;
-  if (int rc = product(R, &xr, gate_up, scale_type, offsets, nullptr, 0, out_dtype, &hr, false, s); rc != SK_OK) return rc;
-  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, out_dtype, nullptr, false, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &xr, gate_up, scale_type, offsets, nullptr, 0, out_dtype, &hr, true, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, out_dtype, nullptr, true, s); rc != SK_OK) return rc;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
   const bool vector = hidden % 8 == 0 && ld_out % 8 == 0 && aligned(out, 16);

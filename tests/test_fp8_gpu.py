@@ -281,6 +281,25 @@ def test_linear_layers():
     assert sk.fp8_linear(v, w_q, w_s).shape == (520,)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("split", [0, 1, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 8), (1, 4096, 4096), (7, 200, 136), (16, 384, 1000), (17, 130, 2056), (32, 1000, 128), (9, 12800, 520), (33, 256, 512)])
+def test_linear_layers_of_few_rows_are_quantiser_and_product(M, N, K, split, dtype, forced):
+    """The bits are those of the two calls, whatever reads the rows (aligned or not), values that are not finite and zeros included."""
+    forced(split=split)
+    g = F.generator(M + K)
+    w_q, w_s = sk.prepare_weight_fp8(torch.randn(N, K, generator=g, device="cuda") * K ** -0.5)
+    wide = F.random_rows(g, M, K + 16, dtype)
+    wide[0, 8:70] = 0
+    if M > 4:
+        wide[1, 9], wide[2, K + 7], wide[3] = float("nan"), float("inf"), 0
+    for lo in (0, 8, 3):
+        x = wide[:, lo:lo + K]
+        y = sk.fp8_linear(x, w_q, w_s)
+        want = sk.fp8_gemm(*sk.quantize_fp8(x), w_q, w_s, dtype)
+        assert torch.equal(torch.nan_to_num(y, 7.0), torch.nan_to_num(want, 7.0)) and torch.equal(torch.isnan(y), torch.isnan(want))
+
+
 def test_refusals():
     x_q, x_s, w_q, w_s = _operands(8, 128, 256, F32, 1)
     e_s = torch.ones(1, 2, device="cuda").to(E8M0)
@@ -466,6 +485,18 @@ def test_a_copy_that_never_lands_ends_in_a_status(M, kernel, scales, forced):
     assert sk.fp8_device_status() == 0
     forced(kernel=kernel)
     assert torch.equal(sk.fp8_gemm(*x), want)
+
+
+def test_a_copy_that_never_lands_ends_in_a_status_in_a_linear_layer(forced):
+    w = sk.prepare_weight_fp8(torch.randn(256, 1024, device="cuda"))
+    x = torch.randn(5, 1024, device="cuda").half()
+    want = sk.fp8_linear(x, *w)
+    forced(limit=2_000_000, skip=3)
+    sk.fp8_linear(x, *w)
+    torch.cuda.synchronize()
+    assert sk.fp8_device_status() != 0
+    forced()
+    assert torch.equal(sk.fp8_linear(x, *w), want)
 
 
 @pytest.mark.skipif("not __import__('torch').cuda.is_available() or __import__('torch').cuda.device_count() < 2", reason="needs two GPUs")
