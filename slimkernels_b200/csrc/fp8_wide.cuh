@@ -259,41 +259,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           const float inv = pow2f(-e);
           uint8_t* dst = static_cast<uint8_t*>(p.out) + m * p.ld_out + n0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int i = 16 * c + 4 * j;
-              w[j] = bad ? 0x7f7f7f7fu : e4m3x2(acc[i] * inv, acc[i + 1] * inv) | (e4m3x2(acc[i + 2] * inv, acc[i + 3] * inv) << 16);
-            }
-            if (n0 + 16 * c + 16 <= p.N) {          // (rows of codes start on 16 bytes)
-              *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (n0 + 16 * c + j < p.N) dst[16 * c + j] = static_cast<uint8_t>(w[j >> 2] >> (8 * (j & 3)));
-            }
-          }
+          for (int c = 0; c < 2; ++c) store_codes32(dst + 32 * c, p.N - n0 - 32 * c, inv, bad, [&](int j) { return acc[32 * c + j]; });
           if (wg == 0) store_scale<false>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
         }
       } else if (live) {
         const int n0 = t.n * 256 + wg * 128;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + m * p.ld_out + n0;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          if (p.vector_out && n0 + 8 * c + 8 <= p.N) {
-            uint4 v;
-            v.x = pack_out(acc[8 * c], acc[8 * c + 1], p.out_bf16);
-            v.y = pack_out(acc[8 * c + 2], acc[8 * c + 3], p.out_bf16);
-            v.z = pack_out(acc[8 * c + 4], acc[8 * c + 5], p.out_bf16);
-            v.w = pack_out(acc[8 * c + 6], acc[8 * c + 7], p.out_bf16);
-            *reinterpret_cast<uint4*>(dst + 8 * c) = v;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (n0 + 8 * c + j < p.N) dst[8 * c + j] = round_out(acc[8 * c + j], p.out_bf16);
-          }
-        }
+        for (int c = 0; c < 8; ++c) store_row16(dst + 16 * c, p.N - n0 - 16 * c, p.vector_out, p.out_bf16, [&](int j) { return acc[16 * c + j]; });
       }
     }
     __syncwarp();

@@ -303,7 +303,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   p.k_blocks = static_cast<int>(ceil_div(K, 128));
   p.n_tiles = static_cast<int>(ceil_div(N, c.feature_tile));
   p.out_bf16 = out_dtype == SK_OUT_BF16;
-  p.vector_out = !silu && aligned(out, 16) && ld_out % 8 == 0;
+  p.vector_out = !silu && aligned(out, 32) && ld_out % 16 == 0;
   const int64_t four = 4 * scale_bytes(scale_type);
   p.x_scale_groups = p.xs_blk == 1 && p.xs_row % 4 == 0 && aligned(p.x_scale, four);
   p.w_scale_groups = p.k_blocks % 4 == 0 && aligned(p.w_scale, four);
@@ -358,15 +358,15 @@ int quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t K, cons
   });
 }
 
-// Codes and scales of [M, K] in a workspace.  The scales lie row by row, rows padded to four: the products read four K blocks' at once.
+// Codes and scales of [M, K] in a workspace, rows on 32 bytes.  The scales lie row by row, rows padded to four: the products read four K blocks' at once.
 int64_t scale_pitch(int64_t K) { return round_up(ceil_div(K, 128), 4); }
 int64_t rows_bytes(int64_t M, int64_t K, int scale_type) {
-  return round_up(M * round_up(K, 16), 256) + round_up(M * scale_pitch(K) * scale_bytes(scale_type), 256);
+  return round_up(M * round_up(K, 32), 256) + round_up(M * scale_pitch(K) * scale_bytes(scale_type), 256);
 }
 sk_fp8_rows rows_in(uint8_t* at, int64_t M, int64_t K, int scale_type) {
   sk_fp8_rows r;
   r.q = at;
-  r.ld = round_up(K, 16);
+  r.ld = round_up(K, 32);
   r.scale = at + round_up(M * r.ld, 256);
   r.scale_row = scale_pitch(K);
   r.scale_block = 1;
@@ -554,7 +554,7 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
 
 int64_t sk_fp8_experts_workspace_bytes(int64_t T, int64_t k, int64_t hidden, int64_t inter, int scale_type) {
   if (T < 0 || k < 1 || hidden < 1 || inter < 1 || !is_scale_type(scale_type)) return 0;
-  return rows_bytes(T * k, hidden, scale_type) + rows_bytes(T * k, inter, scale_type) + round_up(T * k * round_up(hidden, 8) * 2, 256);
+  return rows_bytes(T * k, hidden, scale_type) + rows_bytes(T * k, inter, scale_type) + round_up(T * k * round_up(hidden, 16) * 2, 256);
 }
 
 int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x, const int32_t* rows, const float* weights, const int32_t* offsets,
@@ -571,7 +571,7 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
   if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(workspace, 256)) return SK_ERR_BAD_ALIGNMENT;
   if (T == 0) return SK_OK;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t R = T * k, ld_y = round_up(hidden, 8);
+  const int64_t R = T * k, ld_y = round_up(hidden, 16);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   const sk_fp8_rows xr = rows_in(at, R, hidden, scale_type);
   at += rows_bytes(R, hidden, scale_type);
