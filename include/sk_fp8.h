@@ -80,7 +80,7 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
 
 /* The expert layers of a mixture-of-experts block on routed tokens:
  *   y_e(x) = W_down[e] q( SiLU(gate) * up ),   [gate; up] = W_gate_up[e] q(x),   q the quantiser above,
- *   out[t] = cast( sum_j weights[t, j] * y_{expert of (t, j)}(x[t]) ),   choices with rows < 0 count nothing.
+ *   out[t] = cast( sum_j weights[t, j] * y_{expert of (t, j)}(x[t]) ),   choices with rows outside [0, T * k) count nothing.
  * gate_up: 2 * experts matrices [inter, hidden] (an expert's gate, then its up; `experts` there counts matrices), down: experts
  * matrices [hidden, inter].  y is rounded to out_dtype before it is summed.  x_type: fp16 or bf16 or fp32. */
 int64_t sk_fp8_experts_workspace_bytes(int64_t T, int64_t k, int64_t hidden, int64_t inter, int scale_type);
@@ -92,7 +92,7 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
  * non-zero maps to SK_ERR_DEVICE_TIMEOUT.  sk_device_status_string words it.  The output of such a launch is undefined. */
 int sk_fp8_last_device_status(int device, int* device_status);
 typedef enum sk_fp8_kernel {
-  SK_FP8_KERNEL_FEW = 1,        /* few rows: features on the tensor memory's lanes, tiles of 16, 32 or (8-bit scales) 64 rows */
+  SK_FP8_KERNEL_FEW = 1,        /* few rows: features on the tensor memory's lanes, tiles of 16 or (8-bit scales) 32 rows */
   SK_FP8_KERNEL_MANY = 2,       /* many rows: 128 of them on the lanes */
   SK_FP8_KERNEL_PAIR = 3        /* the same on pairs of CTAs, 256 rows (8-bit scales) */
 } sk_fp8_kernel;                /* 8-bit scales are multiplied in by the tensor core, 32-bit ones in fp32 after every K block */
@@ -103,7 +103,7 @@ int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int sc
 
 /* Testing and tuning, process-wide; 0 restores the default. */
 typedef enum sk_fp8_option {
-  SK_FP8_OPT_ROW_TILE = 1,          /* rows per tile of the kernel for few rows: 16 / 32 / 64 (32 where there is no 64) */
+  SK_FP8_OPT_ROW_TILE = 1,          /* rows per tile of the kernel for few rows: 16 / 32 (16 where there is no 32) */
   SK_FP8_OPT_SPLIT_K = 2,           /* CTAs that share the K range of a tile (products of one group) */
   SK_FP8_OPT_WAIT_LIMIT_CYCLES = 3, /* as SK_OPT_WAIT_LIMIT_CYCLES */
   SK_FP8_OPT_TEST_SKIP_COPY = 4,    /* as SK_OPT_TEST_SKIP_COPY */

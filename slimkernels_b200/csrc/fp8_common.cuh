@@ -35,7 +35,7 @@ struct Fp8Params {
   int up_block0;
   int out_bf16;
   int x_scale_groups, w_scale_groups;   // the scales of four K blocks may be loaded at once (side by side and aligned)
-  int vector_out;                       // rows of the result start on 32 bytes
+  int out_bytes;                        // what the rows of the result start on: 32, 16 or 2 bytes
   int early_weights;                    // the weights may be read before the previous kernel is complete
   int stages;                           // depth of the ring (kernels whose launch decides it)
   int split;                            // CTAs of a cluster that share the K range of a tile
@@ -231,14 +231,19 @@ __device__ __forceinline__ void st_global_v8(void* dst, const uint32_t (&w)[8]) 
                "r"(w[6]), "r"(w[7])
                : "memory");
 }
-// 16 neighbouring results of a row, of which those in front of `left` exist; whole: the row's pieces of 16 start on 32 bytes.
+// 16 neighbouring results of a row, of which those in front of `left` exist.  bytes: what the row's pieces of 16 start on, 32, 16 or less.
 template <class Value>
-__device__ __forceinline__ void store_row16(uint16_t* dst, int left, bool whole, bool bf16, Value&& value) {
-  if (whole && left >= 16) {
+__device__ __forceinline__ void store_row16(uint16_t* dst, int left, int bytes, bool bf16, Value&& value) {
+  if (bytes >= 16 && left >= 16) {
     uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = pack_out(value(2 * j), value(2 * j + 1), bf16);
-    st_global_v8(dst, w);
+    if (bytes == 32) {
+      st_global_v8(dst, w);
+    } else {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 16; ++j)

@@ -45,53 +45,70 @@ __device__ __forceinline__ void load_eight(const void* p, long long i, float (&f
   }
 }
 
+// Eight of a block's 128 values in each of 16 neighbouring lanes -> their codes, the block's exponent and whether it holds a value that is not
+// finite (then the codes are NaN).
+__device__ __forceinline__ uint2 quantise_eight(const float (&f)[8], int* exponent, bool* not_finite) {
+  uint32_t a = 0;                                   // bits of |x|: ordered like the values, infinity and NaN above all
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(f[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const bool bad = not_finite_bits(a);
+  const int e = bad ? 0 : fp8_block_exponent(a);
+  const float inv = pow2f(-e);
+  uint2 code;
+  code.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
+  code.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
+  if (bad) code = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+  *exponent = e;
+  *not_finite = bad;
+  return code;
+}
+
 // x [M, K] -> codes [M, ld_q] and scales, one per row and block of 128 (the rule is fp8_block_exponent's; a block with a value that
 // is not finite has a NaN scale and NaN codes).  Blocks do not depend on one another: 16 lanes hold one, eight elements each.
-// rows != nullptr: row t is written to the rows rows[t * choices .. t * choices + choices - 1] of the result instead (those >= 0),
-// which orders tokens by expert on the way.
+// rows != nullptr: row t is written to the rows rows[t * choices .. t * choices + choices - 1] of the result instead, which orders tokens by expert
+// on the way.  Places outside [0, places) are nobody's.
 template <int TYPE, bool E8M0, bool VECTOR>
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(const void* x, long long ld_x, long long M, int K, uint8_t* q, long long ld_q, void* scale, long long s_row,
-                    long long s_blk, const int* rows, int choices) {
+                    long long s_blk, const int* rows, int choices, int places) {
   // The next kernel may start only when every CTA of this one has passed the wait: what it then reads early (weights) was complete
   // before this kernel's inputs were.
   grid_dep_wait();
   grid_dep_launch_dependents();
-  const int kb = (K + kFp8Block - 1) / kFp8Block;
-  const long long total = M * kb;
-  const int l16 = threadIdx.x & 15;
-  for (long long first = blockIdx.x * 16ll; first < total; first += gridDim.x * 16ll) {   // (whole warps stay together)
-    const long long unit = first + (threadIdx.x >> 4);
-    const bool on = unit < total;
-    const long long m = on ? unit / kb : 0;
-    const int b = on ? static_cast<int>(unit - m * kb) : 0;
-    const int k0 = b * kFp8Block + l16 * 8;
+  // A CTA takes 16 neighbouring blocks (blockIdx.y) of every gridDim.x-th row, two rows a turn; a row's destinations come with its values, one
+  // per lane.
+  const int l16 = threadIdx.x & 15, b = blockIdx.y * 16 + (threadIdx.x >> 4), k0 = b * kFp8Block + l16 * 8;
+  const bool mine = k0 - l16 * 8 < K;               // (past the row's last block: only along for the shuffles)
+  struct Row {
+    long long m;
+    int place;
     float f[8];
-    if (VECTOR && on && k0 + 8 <= K) {
-      load_eight<TYPE>(x, m * ld_x + k0, f);
+  };
+  const auto load = [&](long long m) {
+    Row u;
+    u.m = m < M && mine ? m : -1;
+    u.place = rows != nullptr && u.m >= 0 && l16 < choices ? ld_global_int(rows + m * choices + l16) : -1;
+    if (VECTOR && u.m >= 0 && k0 + 8 <= K) {
+      load_eight<TYPE>(x, m * ld_x + k0, u.f);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = on && k0 + j < K ? load_element<TYPE>(x, m * ld_x + k0 + j) : 0.f;
+      for (int j = 0; j < 8; ++j) u.f[j] = u.m >= 0 && k0 + j < K ? load_element<TYPE>(x, m * ld_x + k0 + j) : 0.f;
     }
-    uint32_t a = 0;                                 // bits of |x|: ordered like the values, infinity and NaN above all
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(f[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if (!on) continue;
-    const bool bad = not_finite_bits(a);
-    const int e = bad ? 0 : fp8_block_exponent(a);
-    const float inv = pow2f(-e);
-    uint2 code;
-    code.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
-    code.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
-    if (bad) code = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+    return u;
+  };
+  const auto store = [&](const Row& u) {
+    int e;
+    bool bad;
+    const uint2 code = quantise_eight(u.f, &e, &bad);
     for (int c = 0; c < choices; ++c) {
-      long long r = m;
+      long long r = u.m;
       if (rows != nullptr) {
-        r = ld_global_int(rows + m * choices + c);
-        if (r < 0) continue;
+        r = __shfl_sync(0xffffffffu, u.place, c & 15, 16);
+        if (c >= 16) r = u.m >= 0 ? ld_global_int(rows + u.m * choices + c) : -1;
       }
+      if (r < 0 || (rows != nullptr && r >= places)) continue;
       uint8_t* dst = q + r * ld_q + k0;
       if (k0 + 8 <= K) {                            // (ld_q is a multiple of 16)
         *reinterpret_cast<uint2*>(dst) = code;
@@ -101,6 +118,11 @@ fp8_quantize_kernel(const void* x, long long ld_x, long long M, int K, uint8_t* 
       }
       if (l16 == 0) store_scale<E8M0>(scale, r * s_row + b * s_blk, e, bad);
     }
+  };
+  for (long long m = blockIdx.x; m < M; m += 2 * gridDim.x) {
+    const Row u0 = load(m), u1 = load(m + gridDim.x);
+    store(u0);
+    store(u1);
   }
 }
 
@@ -149,7 +171,7 @@ fp8_prepare_weight_kernel(const void* w, long long ld_w, long long matrix, int N
   if (threadIdx.x == 0) store_scale<E8M0>(scale, (static_cast<long long>(blockIdx.y) * nb + r) * kb + b, e, bad);
 }
 
-// out[t, :] = round( sum over j of weights[t, j] * y[rows[t, j], :] ), in the order of j; choices with rows < 0 count nothing.
+// out[t, :] = round( sum over j of weights[t, j] * y[rows[t, j], :] ), in the order of j; choices with rows outside [0, T * choices) count nothing.
 template <bool BF16, bool VECTOR>
 __global__ void __launch_bounds__(256)
 fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const float* weights, int choices, int T, int H, uint16_t* out,
@@ -165,7 +187,7 @@ fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const flo
     float acc[8] = {};
     for (int j = 0; j < choices; ++j) {
       const int r = ld_global_int(rows + t * choices + j);
-      if (r < 0) continue;
+      if (r < 0 || r >= T * choices) continue;
       const float w = ld_global_f32(weights + t * choices + j);
       if constexpr (VECTOR) {
         float f[8];
@@ -196,7 +218,7 @@ fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const flo
 //   pass 1  (TOPK: the k largest logits of each token and their weights) and how many choices each expert got from this CTA
 //   pass 2  (after pass 1 of all CTAs) the experts' first rows, and the place of each choice
 // With one CTA both are one launch.  Latency bounds all of it (8192 tokens of 256 logits are 4 MB): 32 warps to a CTA, a token's logits
-// loaded while the one before it is worked on, and only the lane that held a winner looks through its logits again.
+// loaded while the one before it is worked on.
 constexpr int kRouteWarps = 32;
 struct RouteParams {
   const void* logits;                   // [T, ld]
@@ -221,63 +243,112 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// The logits of one token: lane holds those of experts lane, lane + 32, ...
+// One token: lane holds the logits of experts lane, lane + 32, ...; the choice of a round is the largest left, the lowest expert among equals.
+// A logit of 16 bits and its expert fit one word, so that a round is one reduction and no two words are equal:
+//   bits that order like the logits | 0xffff - expert
+// 32-bit logits take a second reduction where several lanes hold the largest.  Only the lane that held it looks through its logits again.
 template <int TYPE, int PER>
-__device__ __forceinline__ void load_logits(const RouteParams& p, long long t, int lane, float (&f)[PER]) {
-#pragma unroll
-  for (int i = 0; i < PER; ++i) f[i] = lane + 32 * i < p.E ? load_element<TYPE>(p.logits, t * p.ld + lane + 32 * i) : 0.f;
-}
+struct TokenLogits {
+  static constexpr bool kWord = TYPE != 2;
+  uint32_t key[PER];                    // 0: none (below -infinity's)
 
-// The choice of round j is the largest value left, the lowest expert among equals.
-template <int PER>
-__device__ __forceinline__ void choose_experts(const RouteParams& p, long long t, int lane, const float (&f)[PER]) {
-  uint32_t key[PER];
+  static __device__ __forceinline__ uint32_t order16(uint32_t b) {
+    const bool nan = TYPE == 1 ? (b & 0x7fffu) > 0x7f80u : (b & 0x7fffu) > 0x7c00u;
+    if (nan) return 0xffffu;
+    if (b == 0x8000u) b = 0;
+    return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+  }
+  static __device__ __forceinline__ float value16(uint32_t o) {
+    if (o == 0xffffu) return __uint_as_float(0x7fc00000u);
+    const uint32_t b = o & 0x8000u ? o & 0x7fffu : ~o & 0xffffu;
+    if constexpr (TYPE == 1) return __uint_as_float(b << 16);
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+  }
+  static __device__ __forceinline__ float value(uint32_t k) { return kWord ? value16(k >> 16) : from_ordered_bits(k); }
+  static __device__ __forceinline__ bool masked(uint32_t k) {   // -infinity
+    return kWord ? (k >> 16) == (TYPE == 1 ? 0x007fu : 0x03ffu) : k == 0x007fffffu;
+  }
+
+  __device__ __forceinline__ void load(const RouteParams& p, long long t, int lane) {   // as they lie in memory, so that nothing waits yet
 #pragma unroll
-  for (int i = 0; i < PER; ++i) key[i] = lane + 32 * i < p.E ? ordered_bits(f[i]) : 0u;      // (0 is below -infinity's bits)
-  uint32_t best = 0;
-  int at = 0;
-  auto look = [&]() {                   // the lane's own largest; 0: none left
-    best = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
-  };
-  look();
-  float top = 0.f, sum = 0.f, mine = 0.f;
-  uint32_t first_bits = 0;
-  int my_id = 0;
-  for (int j = 0; j < p.k; ++j) {
-    const uint32_t winner = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t holders = __ballot_sync(0xffffffffu, best == winner);
-    int e = __shfl_sync(0xffffffffu, at, __ffs(holders) - 1);
-    if (holders & (holders - 1)) e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
-    if (j == 0) {
-      first_bits = winner;
-      top = from_ordered_bits(winner);
-      if (!p.renormalize) {             // the whole softmax's sum, while all keys are there
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (lane + 32 * i < p.E) sum += expf(from_ordered_bits(key[i]) - top);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int i = 0; i < PER; ++i) {
+      key[i] = 0;
+      if (lane + 32 * i >= p.E) continue;
+      if constexpr (kWord) {
+        unsigned short v;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(static_cast<const uint16_t*>(p.logits) + t * p.ld + lane + 32 * i) : "memory");
+        key[i] = v;
+      } else {
+        key[i] = __float_as_uint(ld_global_f32(static_cast<const float*>(p.logits) + t * p.ld + lane + 32 * i));
       }
     }
-    if ((e & 31) == lane) {
+  }
+  __device__ __forceinline__ void order(const RouteParams& p, int lane) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (lane + 32 * i == e) key[i] = 0;
-      look();
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane + 32 * i;
+      if (e >= p.E) key[i] = 0;
+      else if constexpr (kWord) key[i] = order16(key[i]) << 16 | (0xffffu - e);
+      else key[i] = ordered_bits(__uint_as_float(key[i]));
     }
-    const float w = expf(from_ordered_bits(winner) - top);
-    if (p.renormalize) sum += w;
-    if (lane == j) { mine = w; my_id = e; }
   }
-  if (lane < p.k) {
-    p.ids[t * p.k + lane] = my_id;
-    // a token whose logits are all -infinity has no distribution: its weights are zero
-    p.weights[t * p.k + lane] = first_bits == 0x007fffffu ? 0.f : mine / sum;
+
+  __device__ __forceinline__ void choose(const RouteParams& p, long long t, int lane) {
+    order(p, lane);
+    uint32_t best = 0;
+    int at = 0;
+    auto look = [&]() {                 // the lane's own largest; 0: none left
+      best = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if constexpr (kWord) best = max(best, key[i]);
+        else if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+      }
+    };
+    look();
+    float top = 0.f, sum = 0.f, mine = 0.f;
+    uint32_t first = 0;
+    int my_id = 0;
+    for (int j = 0; j < p.k; ++j) {
+      const uint32_t winner = __reduce_max_sync(0xffffffffu, best);
+      int e;
+      if constexpr (kWord) {
+        e = static_cast<int>(0xffffu - (winner & 0xffffu));
+      } else {
+        const uint32_t holders = __ballot_sync(0xffffffffu, best == winner);
+        e = __shfl_sync(0xffffffffu, at, __ffs(holders) - 1);
+        if (holders & (holders - 1)) e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
+      }
+      if (j == 0) {
+        first = winner;
+        top = value(winner);
+        if (!p.renormalize) {           // the whole softmax's sum, while all keys are there
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (lane + 32 * i < p.E) sum += expf(value(key[i]) - top);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+      }
+      if ((e & 31) == lane) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (kWord ? key[i] == winner : lane + 32 * i == e) key[i] = 0;
+        look();
+      }
+      if (lane == j) { mine = value(winner); my_id = e; }
+    }
+    // lane j holds choice j: its weight, and the sum of all in the order of the choices
+    mine = expf(mine - top);
+    if (p.renormalize)
+      for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, mine, j);
+    if (lane < p.k) {
+      p.ids[t * p.k + lane] = my_id;
+      // a token whose logits are all -infinity has no distribution: its weights are zero
+      p.weights[t * p.k + lane] = masked(first) ? 0.f : mine / sum;
+    }
   }
-}
+};
 
 struct RouteRange { long long t0, t1; };   // tokens of this warp
 __device__ __forceinline__ RouteRange route_range(const RouteParams& p) {
@@ -296,17 +367,13 @@ __device__ __forceinline__ void route_count(const RouteParams& p, int* hist) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const RouteRange r = route_range(p);
   if constexpr (TOPK) {
-    float f[PER];
-    if (r.t0 < r.t1) load_logits<TYPE, PER>(p, r.t0, lane, f);
+    TokenLogits<TYPE, PER> now, next;
+    if (r.t0 < r.t1) now.load(p, r.t0, lane);
     for (int i = threadIdx.x; i < warps * p.E; i += blockDim.x) hist[i] = 0;
     for (long long t = r.t0; t < r.t1; ++t) {
-      float next[PER];
-      if (t + 1 < r.t1) load_logits<TYPE, PER>(p, t + 1, lane, next);
-      choose_experts<PER>(p, t, lane, f);
-      if (t + 1 < r.t1) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) f[i] = next[i];
-      }
+      if (t + 1 < r.t1) next.load(p, t + 1, lane);
+      now.choose(p, t, lane);
+      now = next;
     }
     __syncwarp();
   } else {
@@ -325,10 +392,15 @@ __device__ __forceinline__ void route_place(const RouteParams& p, int* hist, con
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int at = base[e];
-    for (int w = 0; w < warps; ++w) {
-      const int n = hist[w * p.E + e];
-      hist[w * p.E + e] = at;
-      at += n;
+    for (int w0 = 0; w0 < warps; w0 += 8) {         // (eight loads at once: one after another they are a chain of round trips)
+      int n[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n[i] = w0 + i < warps ? hist[(w0 + i) * p.E + e] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (w0 + i < warps) hist[(w0 + i) * p.E + e] = at;
+        at += n[i];
+      }
     }
   }
   __syncthreads();
@@ -348,24 +420,31 @@ __device__ __forceinline__ void route_place(const RouteParams& p, int* hist, con
   }
 }
 
-// Exclusive sums over the experts of total[] (in place -> first places), by warp 0; the grand total is stored behind them.
-__device__ __forceinline__ void scan_experts(int* total, int E) {
-  if (threadIdx.x < 32) {
-    int carry = 0;
-    for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + static_cast<int>(threadIdx.x);
-      const int n = e < E ? total[e] : 0;
-      int incl = n;
+// Exclusive sums over the experts of total[] (in place -> first places); the grand total is stored behind them.  A warp scans 32 experts, then
+// adds what lies in front of them (at most 32 such sums).
+__device__ __forceinline__ int warp_scan(int n, int lane) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (static_cast<int>(threadIdx.x) >= o) incl += up;
-      }
-      if (e < E) total[e] = carry + incl - n;
-      carry += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (threadIdx.x == 0) total[E] = carry;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, n, o);
+    if (lane >= o) n += up;
   }
+  return n;
+}
+__device__ __forceinline__ void scan_experts(int* total, int E) {
+  __shared__ int ahead[32];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = (E + 31) >> 5;
+  for (int g = warp; g < parts; g += warps) {
+    const int e = 32 * g + lane, n = e < E ? total[e] : 0, incl = warp_scan(n, lane);
+    if (e < E) total[e] = incl - n;
+    if (lane == 31) ahead[g] = incl;
+  }
+  __syncthreads();
+  const int part = lane < parts ? ahead[lane] : 0, sums = warp_scan(part, lane);
+  for (int g = warp; g < parts; g += warps) {
+    const int before = __shfl_sync(0xffffffffu, sums - part, g);
+    if (32 * g + lane < E) total[32 * g + lane] += before;
+  }
+  if (threadIdx.x == 31) total[E] = sums;
   __syncthreads();
 }
 

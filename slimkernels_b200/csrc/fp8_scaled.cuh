@@ -358,7 +358,7 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         uint16_t* dst = static_cast<uint16_t*>(p.out) + m * p.ld_out + n0;
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          store_row16(dst + 16 * c, p.N - n0 - 16 * c, p.vector_out, p.out_bf16,
+          store_row16(dst + 16 * c, p.N - n0 - 16 * c, p.out_bytes, p.out_bf16,
                       [&](int j) { return __uint_as_float(v[c >> 1][16 * (c & 1) + j]); });
       }
     }

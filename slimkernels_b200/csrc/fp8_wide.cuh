@@ -266,7 +266,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         const int n0 = t.n * 256 + wg * 128;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + m * p.ld_out + n0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) store_row16(dst + 16 * c, p.N - n0 - 16 * c, p.vector_out, p.out_bf16, [&](int j) { return acc[16 * c + j]; });
+        for (int c = 0; c < 8; ++c) store_row16(dst + 16 * c, p.N - n0 - 16 * c, p.out_bytes, p.out_bf16, [&](int j) { return acc[16 * c + j]; });
       }
     }
     __syncwarp();

@@ -155,14 +155,19 @@ struct Choice {
 };
 
 // What a product, or the products of the groups, are launched as.  Measured on B200 (us; few rows: features on the tensor memory's lanes in tiles
-// of 16 / 32 / 64 rows, many: rows on the lanes, 128 a CTA or 256 a pair of CTAs).
-//   One group, 8-bit scales, K 4096:   64 rows x 12288   few 15.2, many 18.4, pair 18.6      256 x 4096   few 13.6, many 17.1, pair 15.3
-//                                     256 rows x 12288   few 27.3, many 20.9, pair 19.1      512 x 4096   few 16.5, many 17.0, pair 15.7
-//   so few rows' kernel takes up to 128 rows, and more for as long as its tiles of 64 rows fit the SMs at once; the pair takes the rest.
-//   One group, 32-bit scales, K 4096:  64 rows x 12288   few 19.8, many 22.9     128 x 4096   few 14.0, many 22.6     128 x 12288   few 35.7, many 25.4
-//   By expert, 16 experts x 4096 x 2048, 8-bit scales, rows per expert (ragged) 2 / 16 / 64 / 256 / 1024:
-//     few rows, tile 16  21.9 / 26.9 / 41.9     tile 32  22.6 / 26.2 / 34.2     many  27.6 / 26.9 / 28.7 / 53.3 / 148.8     pair  30.4 / 32.9 / 35.7 / 51.6 / 138.5
-//   (a pair's tiles of 256 rows are emptier at a group's end, which costs more than its faster MMAs give up to about 512 rows).
+// of 16 or 32 rows, many: rows on the lanes, 128 a CTA or 256 a pair of CTAs).
+//   One group, 8-bit scales, tile of 32 / many / pair:
+//     K 4096:  64 x 12288  14.2 / 17.1 / 15.4     128 x 12288  21.3 / 17.8 / 16.2     256 x 4096  12.6 / 14.3 / 14.8     512 x 4096  20.7 / 14.7 / 15.2
+//     K 8192:  64 x 8192   18.4 / 29.8 / 23.9     128 x 8192   21.9 / 30.9 / 25.1     256 x 8192  37.6 / 30.7 / 25.2
+//   so few rows' kernel takes what its tiles of 32 rows hold with two CTAs to an SM, and a stream of weights (up to 32 rows) always; the pair the rest.
+//   One group, 32-bit scales, K 4096, tile of 16 / many:  32 x 12288  14.8 / 23.0   64 x 12288  22.4 / 21.8   128 x 4096  12.8 / 20.8   256 x 4096  22.5 / 20.8
+//   By expert, 16 experts x 4096 x 2048, 8-bit scales, rows per expert (ragged) 2 / 8 / 16 / 32 / 64 / 256 / 1024:
+//     tile 16  21.7 / 26.1 / 26.8 / 31.4 / 41.9     tile 32  22.5 / 25.8 / 25.9 / 29.2 / 34.4
+//     many     27.1 / 26.3 / 26.5 / 27.1 / 27.7 / 49.9 / 135.6     pair  30.1 / 31.2 / 32.1 / 33.1 / 34.3 / 48.7 / 126.4
+//   (64 experts x 2048 x 2048 at 16 and 32: tile 32  47.9, 50.3, many  50.2, 51.4).  A pair's tiles of 256 rows are emptier at a group's end, which costs
+//   more than its faster MMAs give up to about 512 rows (expert layers of 512 rows each: many 195, pair 201).  With 32-bit scales, 2 / 16 / 32 / 64:
+//     tile 16  21.9 / 27.0 / 33.4 / 47.8     many  28.7 / 29.8 / 31.0 / 31.4
+//   With the SiLU epilogue, whose time goes with the tile's rows, tiles of 16 are the fastest up to 32 rows per expert (67 us a block, tiles of 32 87, many 80).
 // A tile's K range is split while that leaves an SM for every CTA and a CTA eight K blocks or so: 64 x 4096 x 4096 12.9 us in one, 10.9 in four; splitting
 // where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two).
 Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, int sms) {
@@ -171,13 +176,11 @@ Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bo
   const int64_t blocks = ceil_div(N, 128), kb = ceil_div(K, 128);
   bool few;
   if (grouped) {
-    few = rows <= 32;
+    few = rows <= (e8m0 ? 32 : 16);
     c.row_tile = rows <= 8 ? 16 : 32;
-  } else if (e8m0) {
-    few = rows <= 128 || ceil_div(rows, 64) * blocks <= sms;
-    c.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   } else {
-    few = rows <= 64 || ceil_div(rows, 32) * blocks <= sms;
+    const int tile = e8m0 ? 32 : 16;
+    few = rows <= 32 || ceil_div(rows, tile) * blocks <= 2 * sms;
     c.row_tile = rows <= 16 ? 16 : 32;
   }
   c.kernel = few ? SK_FP8_KERNEL_FEW : !e8m0 || (grouped && rows <= 512) ? SK_FP8_KERNEL_MANY : SK_FP8_KERNEL_PAIR;
@@ -185,7 +188,7 @@ Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bo
   few = c.kernel == SK_FP8_KERNEL_FEW;
   if (few) {
     if (const int64_t forced = g_options[SK_FP8_OPT_ROW_TILE].load()) c.row_tile = static_cast<int>(forced);
-    if (silu || !e8m0) c.row_tile = std::min(c.row_tile, 32);
+    if (silu || !e8m0) c.row_tile = 16;
     c.feature_tile = 128;
   } else {
     c.row_tile = c.kernel == SK_FP8_KERNEL_PAIR ? 256 : 128;
@@ -201,15 +204,15 @@ Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bo
   return c;
 }
 
-template <int TOK, bool SILU>
+template <bool SILU>
 int launch_narrow(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
-  using T = Fp8NarrowTraits<TOK, SILU>;
-  auto kern = fp8_narrow_kernel<TOK, SILU>;
+  using T = Fp8NarrowTraits<SILU>;
+  auto kern = fp8_narrow_kernel<SILU>;
   constexpr int kMost = T::dynamic_bytes(SILU ? 1 : 8, kFp8MaxExperts);
-  static_assert(kMost <= 232448 && T::dynamic_bytes(SILU ? 1 : 8, 1) <= (T::kCtas == 2 ? 115712 : 232448), "shared memory of a CTA");
+  static_assert(kMost <= 232448 && T::dynamic_bytes(SILU ? 1 : 8, 1) <= 115712, "shared memory of a CTA");
   static std::atomic<uint64_t> done;
   if (int rc = allow_shared(kern, kMost, dev, done); rc != SK_OK) return rc;
-  const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * T::kCtas);
+  const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * 2);
   LaunchConfig lc(grid, 1, T::kThreads, T::dynamic_bytes(p.split, p.experts), true, p.split, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
@@ -257,15 +260,13 @@ int launch_product(const Choice& c, bool e8m0, const CUtensorMap& mw, const CUte
                    cudaStream_t stream) {
   if (!e8m0) {
     if (c.kernel == SK_FP8_KERNEL_MANY) return launch_wide<SILU>(mw, mx, p, tiles, dev, stream);
-    if (c.row_tile == 16) return launch_narrow<16, SILU>(mw, mx, p, tiles, dev, stream);
-    return launch_narrow<32, SILU>(mw, mx, p, tiles, dev, stream);
+    return launch_narrow<SILU>(mw, mx, p, tiles, dev, stream);
   }
   if (c.kernel == SK_FP8_KERNEL_MANY) return launch_scaled<1, SILU>(mw, mx, p, tiles, dev, stream);
   if (c.kernel == SK_FP8_KERNEL_PAIR) return launch_scaled<2, SILU>(mw, mx, p, tiles, dev, stream);
-  if (c.row_tile == 16) return launch_scaled_narrow<16, SILU>(mw, mx, p, tiles, dev, stream);
   if constexpr (!SILU)
-    if (c.row_tile == 64) return launch_scaled_narrow<64, SILU>(mw, mx, p, tiles, dev, stream);
-  return launch_scaled_narrow<32, SILU>(mw, mx, p, tiles, dev, stream);
+    if (c.row_tile == 32) return launch_scaled_narrow<32, SILU>(mw, mx, p, tiles, dev, stream);
+  return launch_scaled_narrow<16, SILU>(mw, mx, p, tiles, dev, stream);
 }
 
 // silu_out: the SiLU epilogue; w then holds 2 * experts matrices of N rows.  early_weights: this library's quantiser is in front, or a product
@@ -303,7 +304,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   p.k_blocks = static_cast<int>(ceil_div(K, 128));
   p.n_tiles = static_cast<int>(ceil_div(N, c.feature_tile));
   p.out_bf16 = out_dtype == SK_OUT_BF16;
-  p.vector_out = !silu && aligned(out, 32) && ld_out % 16 == 0;
+  p.out_bytes = silu ? 32 : aligned(out, 32) && ld_out % 16 == 0 ? 32 : aligned(out, 16) && ld_out % 8 == 0 ? 16 : 2;
   const int64_t four = 4 * scale_bytes(scale_type);
   p.x_scale_groups = p.xs_blk == 1 && p.xs_row % 4 == 0 && aligned(p.x_scale, four);
   p.w_scale_groups = p.k_blocks % 4 == 0 && aligned(p.w_scale, four);
@@ -341,18 +342,19 @@ int quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t K, cons
              int64_t choices, cudaStream_t stream) {
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
-  const int64_t units = M * ceil_div(K, 128);
-  const int64_t grid = std::min<int64_t>(ceil_div(units, 16), static_cast<int64_t>(dev.sms) * 8);
+  const int64_t parts = ceil_div(ceil_div(K, 128), 16), most = std::max<int64_t>(1, static_cast<int64_t>(dev.sms) * 8 / parts);
+  if (parts > 65535) return SK_ERR_BAD_SHAPE;
   const int64_t size = x_type == SK_FLOAT_F32 ? 4 : 2;
   const bool vector = aligned(x, 16) && ld_x * size % 16 == 0;
-  LaunchConfig lc(grid, 1, 256, 0, true, 1, stream);
+  LaunchConfig lc(std::min(M, most), parts, 256, 0, true, 1, stream);
   return with_type(x_type, [&](auto type) {
     return with_bool(scale_type == SK_SCALE_E8M0, [&](auto e8m0) {
       return with_bool(vector, [&](auto v) {
         return cuda_status(cudaLaunchKernelEx(&lc.cfg, fp8_quantize_kernel<decltype(type)::value, decltype(e8m0)::value, decltype(v)::value>, x,
                                               static_cast<long long>(ld_x), static_cast<long long>(M), static_cast<int>(K), out.q,
                                               static_cast<long long>(out.ld), out.scale, static_cast<long long>(out.scale_row),
-                                              static_cast<long long>(out.scale_block), static_cast<const int*>(rows), static_cast<int>(choices)));
+                                              static_cast<long long>(out.scale_block), static_cast<const int*>(rows), static_cast<int>(choices),
+                                              static_cast<int>(std::min<int64_t>(M * choices, kIntMax))));
       });
     });
   });
@@ -544,7 +546,7 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
                        sk_stream_t stream) {
   if (!ids || !rows || !offsets) return SK_ERR_NULL_POINTER;
   if (int rc = check_route(T, E, 1); rc != SK_OK) return rc;
-  if (k < 1 || k > 1024) return SK_ERR_BAD_SHAPE;
+  if (k < 1 || k > 1024 || T * k > kIntMax) return SK_ERR_BAD_SHAPE;
   RouteParams p = {};
   p.ids = const_cast<int32_t*>(ids);               // (only read)
   p.rows = rows;
@@ -628,7 +630,7 @@ int sk_fp8_set_option(int key, int64_t value) {
   if (value < 0) return SK_ERR_BAD_ARGUMENT;
   switch (key) {
     case SK_FP8_OPT_ROW_TILE:
-      if (value != 0 && value != 16 && value != 32 && value != 64) return SK_ERR_BAD_ARGUMENT;
+      if (value != 0 && value != 16 && value != 32) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_SPLIT_K:
       if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return SK_ERR_BAD_ARGUMENT;

@@ -129,6 +129,8 @@ def test_router_and_experts_refuse_bad_arguments(built_libs):
     assert lib.sk_group_by_expert(None, 4, 2, 8, FAKE, FAKE, FAKE, 1 << 20, None) == capi.SK_ERR_NULL_POINTER
     assert lib.sk_group_by_expert(FAKE, 4, 2, 0, FAKE, FAKE, FAKE, 1 << 20, None) == capi.SK_ERR_BAD_SHAPE
 
+    assert lib.sk_group_by_expert(FAKE, 1 << 24, 1024, 8, FAKE, FAKE, FAKE, 1 << 40, None) == capi.SK_ERR_BAD_SHAPE      # places past 31 bits
+
     need = lib.sk_fp8_experts_workspace_bytes(4, 2, 128, 256, 0)
 
     def experts(T=4, k=2, x=FAKE, gate_up=None, down=None, ws=need, out=FAKE):
@@ -147,7 +149,7 @@ def test_router_and_experts_refuse_bad_arguments(built_libs):
 def test_options_are_checked(built_libs):
     from slimkernels_b200 import capi
     lib = capi.load()
-    for key, value in [(1, 48), (1, -1), (2, 3), (3, 10), (0, 0), (99, 0), (5, 4), (1, 128)]:
+    for key, value in [(1, 48), (1, -1), (2, 3), (3, 10), (0, 0), (99, 0), (5, 4), (1, 64)]:
         assert lib.sk_fp8_set_option(key, value) == capi.SK_ERR_BAD_ARGUMENT, (key, value)
     for key in (1, 2, 3, 4, 5):
         assert lib.sk_fp8_set_option(key, 0) == capi.SK_OK

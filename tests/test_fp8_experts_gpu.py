@@ -184,7 +184,7 @@ def test_expert_layers(T, E, k, hidden, inter, dtype, scales):
     assert torch.equal(y, sk.fp8_experts(x, routing, *gu, *dn))
 
 
-@pytest.mark.parametrize("kernel,row_tile", [(capi.FP8_FEW, 16), (capi.FP8_FEW, 32), (capi.FP8_MANY, 0), (capi.FP8_PAIR, 0)])
+@pytest.mark.parametrize("kernel,row_tile", [(capi.FP8_FEW, 0), (capi.FP8_MANY, 0), (capi.FP8_PAIR, 0)])
 @pytest.mark.parametrize("hidden,inter,scales", [(384, 256, E8M0), (144, 300, F32), (272, 144, E8M0), (256, 1111, F32)])
 def test_expert_layers_every_kernel(kernel, row_tile, hidden, inter, scales):
     T, E, k = 500, 5, 2
@@ -234,6 +234,19 @@ def test_choices_of_experts_that_are_not_here():
     assert bool((y[3] == 0).all())
     rows, offsets = sk.group_by_expert(ids * 0 - 1, E)
     assert bool((sk.fp8_experts(x, sk.Routing(ids, weights, rows, offsets), *gu, *dn) == 0).all())
+
+
+def test_places_outside_the_rows_count_nothing():
+    T, E, k, hidden, inter = 10, 3, 2, 128, 128
+    g, gu, dn = _layers(E, hidden, inter, E8M0, 6)
+    x = F.random_rows(g, T, hidden, torch.float16)
+    r = sk.route_tokens(torch.randn(T, E, generator=g, device="cuda"), k)
+    rows = r.rows.clone()
+    rows[2, 0], rows[5, 1], rows[6, 0] = T * k, 2 ** 31 - 1, -(2 ** 31)
+    y = sk.fp8_experts(x, r._replace(rows=rows), *gu, *dn)
+    weights = r.weights.clone()
+    weights[2, 0] = weights[5, 1] = weights[6, 0] = 0
+    assert torch.equal(y, sk.fp8_experts(x, r._replace(weights=weights), *gu, *dn))
 
 
 def test_a_broken_token_leaves_the_others_alone():

@@ -158,7 +158,7 @@ def test_product_at_working_sizes(M, N, K, scales):
     _check_product(*_operands(M, N, K, scales, M + N + K), torch.bfloat16)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64])
+@pytest.mark.parametrize("row_tile", [16, 32])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 2048), (130, 200, 1100), (257, 1024, 1024)])
 @pytest.mark.parametrize("scales", [E8M0, F32])
@@ -182,7 +182,7 @@ def test_every_kernel(M, N, K, kernel, scales, forced):
     assert torch.equal(y, sk.fp8_gemm(*x, torch.float16))
 
 
-@pytest.mark.parametrize("row_tile", [0, 16, 32, 64])
+@pytest.mark.parametrize("row_tile", [0, 16, 32])
 @pytest.mark.parametrize("kernel", [capi.FP8_FEW, capi.FP8_MANY, capi.FP8_PAIR])
 def test_every_scale_reaches_its_row_and_block(kernel, row_tile, forced):
     """Scales that differ from row to row and block to block by large factors, in any memory order: none may be taken for another's."""
@@ -356,7 +356,7 @@ def test_grouped_product(offsets, N, K, scales, out_dtype):
     _check_grouped(offsets, offsets[-1] + 9, N, K, scales, out_dtype)
 
 
-@pytest.mark.parametrize("row_tile", [16, 32, 64])
+@pytest.mark.parametrize("row_tile", [16, 32])
 @pytest.mark.parametrize("scales", [E8M0, F32])
 def test_grouped_product_of_few_rows_every_tile(scales, row_tile, forced):
     forced(row_tile, kernel=capi.FP8_FEW)
