@@ -291,11 +291,11 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           const uint32_t sb[8] = {w[0], w[0], w[0], w[0], w[1], w[1], w[1], w[1]};
           tmem_st_32x4(t_lane + slot * T::kSlotCols, sa);
           tmem_st_32x8(t_lane + slot * T::kSlotCols + 4, sb);
-          if (g + 1 < groups_of_four) fetch(4 * g + 4);
           tmem_st_wait();
           tcgen05_fence_before_sync();
           __syncwarp();
           if (lane == 0) arrive_first<CTAS>(bar_scales + 8 * slot);
+          if (g + 1 < groups_of_four) fetch(4 * g + 4);      // (scales read byte by byte are waited for: nobody else should)
           if (++slot == T::kSlots) { slot = 0; phase ^= 1; }
         }
       }

@@ -236,11 +236,11 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
 #pragma unroll
         for (int i = 0; i < 4; ++i) sb[i] = x[i < T::kXCols ? i : 0];
         tmem_st_32x4(at + 4 * kW, sb);
-        if (kb + 4 < kb_end) fetch(kb + 4);
         tmem_st_wait();
         tcgen05_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_scales + 8 * slot);
+        if (kb + 4 < kb_end) fetch(kb + 4);         // (scales read byte by byte are waited for: nobody else should)
         if (++slot == T::kSlots) { slot = 0; phase ^= 1; }
       }
     }

@@ -1,4 +1,5 @@
 """The FP8 quantisers and products on the GPU against their definition in 64 bits (tolerances: fp8_util)."""
+import ctypes
 import subprocess
 import sys
 
@@ -199,6 +200,30 @@ def test_every_scale_reaches_its_row_and_block(kernel, row_tile, forced):
     assert turned.stride() == (1, M)
     for other in (turned, wide[:, 1:].view(E8M0)):
         assert torch.equal(y, sk.fp8_gemm(x_q, other, w_q, w_s))
+
+
+def test_launches_are_what_the_rules_say(forced):
+    lib = capi.load()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+
+    def query(M, N, K, E=1, scales=E8M0):
+        v = [ctypes.c_int() for _ in range(5)]
+        assert lib.sk_fp8_query_launch(M, N, K, E, capi.SK_SCALE_E8M0 if scales == E8M0 else capi.SK_SCALE_F32, *map(ctypes.byref, v)) == 0
+        return [i.value for i in v]
+
+    assert query(1, 4096, 4096)[:4] == [capi.FP8_FEW, 16, 128, 4]
+    assert query(17, 57344, 8192)[:4] == [capi.FP8_FEW, 32, 128, 1]
+    assert query(256, 4096, 4096)[:3] == [capi.FP8_FEW, 32, 128] and query(4096, 4096, 4096)[:4] == [capi.FP8_PAIR, 256, 256, 1]
+    assert query(64, 4096, 4096, scales=F32)[:3] == [capi.FP8_FEW, 16, 128] and query(512, 4096, 4096, scales=F32)[:3] == [capi.FP8_MANY, 128, 256]
+    assert query(64, 2048, 2048, 64)[:3] == [capi.FP8_FEW, 16, 128] and query(64 * 20, 2048, 2048, 64)[:3] == [capi.FP8_FEW, 32, 128]
+    assert query(64 * 100, 2048, 2048, 64)[:3] == [capi.FP8_MANY, 128, 256] and query(64 * 600, 2048, 2048, 64)[:3] == [capi.FP8_PAIR, 256, 256]
+    assert query(64 * 20, 2048, 2048, 64, F32)[0] == capi.FP8_MANY
+    kernel, tile, features, split, ctas = query(5, 1024, 8192)
+    assert ctas == 8 * split and ctas <= sms and split == 8
+    for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 1, 2000)):
+        assert lib.sk_fp8_query_launch(*bad, 0, None, None, None, None, None) == capi.SK_ERR_BAD_SHAPE
+    forced(kernel=capi.FP8_PAIR)
+    assert query(5, 1024, 8192)[0] == capi.FP8_PAIR and query(5, 1024, 8192, scales=F32)[0] == capi.FP8_MANY
 
 
 def test_product_strides():
