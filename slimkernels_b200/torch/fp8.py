@@ -115,9 +115,30 @@ def _padded_codes(w, scale_dtype):
     return full, scale
 
 
-class FP8Linear(nn.Module):
+class _KeepsTypes(nn.Module):
+    """Codes and scales are moved as they are: `.half()` and `.to(dtype)` are for what a model computes in, not for them."""
+
+    _as_they_are = ()
+
+    def _apply(self, fn, recurse=True):
+        held = {name: self._buffers[name] for name in self._as_they_are}
+        for name in held:
+            self._buffers[name] = None
+        try:
+            super()._apply(fn, recurse)
+            moved = {name: fn(t.view(torch.uint8 if t.element_size() == 1 else torch.int32)).view(t.dtype) for name, t in held.items()}
+        except BaseException:
+            self._buffers.update(held)
+            raise
+        self._buffers.update(moved)
+        return self
+
+
+class FP8Linear(_KeepsTypes):
     """y = x W^T (+ bias) with an 8-bit weight and activations quantised on the way.  w_q float8_e4m3fn [out_features, in_features
     padded to a multiple of 16], w_scale [ceil(out / 128), ceil(in / 128)]."""
+
+    _as_they_are = ("w_q", "w_scale")
 
     def __init__(self, w_q, w_scale, in_features, bias=None, out_dtype=torch.float16):
         super().__init__()
@@ -134,14 +155,16 @@ class FP8Linear(nn.Module):
 
     def forward(self, x):
         y = fp8_linear(x, self.w_q[:, :self.in_features], self.w_scale, self.out_dtype)
-        return y if self.bias is None else y + self.bias
+        return y if self.bias is None else y + self.bias.to(y.dtype)
 
 
-class FP8Experts(nn.Module):
+class FP8Experts(_KeepsTypes):
     """The expert layers of a mixture-of-experts block with 8-bit weights: `fp8_experts` on tokens routed by the caller.
 
     gate_up [E, 2, inter, hidden padded to 16], down [E, hidden, inter padded to 16] and their scales.
     """
+
+    _as_they_are = ("gate_up", "gate_up_scale", "down", "down_scale")
 
     def __init__(self, gate_up, gate_up_scale, down, down_scale, hidden, inter, out_dtype=torch.float16):
         super().__init__()

@@ -120,3 +120,22 @@ def test_what_is_no_stack_of_experts_is_left_alone():
     assert sk.quantize_linears(model, skip=("lm_head", "gate"), experts=True) == {"linear": 0, "mlp": 0, "kept": ["moe.gate", "lm_head"], "experts": 0}
     assert isinstance(model.moe.experts, _Experts)
 
+
+
+@pytest.mark.parametrize("scales", [E8M0, F32])
+def test_casts_of_a_model_leave_codes_and_scales_alone(scales):
+    torch.manual_seed(6)
+    lin = sk.FP8Linear.from_float(torch.randn(130, 200), torch.randn(130), out_dtype=torch.bfloat16, scale_dtype=scales)
+    experts = sk.FP8Experts.from_float(torch.randn(3, 96, 64), torch.randn(3, 64, 48), scale_dtype=scales)
+    x, z = torch.randn(7, 200, device="cuda"), torch.randn(7, 64, device="cuda")
+    ids, weights = torch.randint(0, 3, (7, 2), device="cuda"), torch.rand(7, 2, device="cuda")
+    plain = sk.fp8_linear(x, lin.w_q[:, :200], lin.w_scale, torch.bfloat16)
+    want = experts(z, ids, weights)
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.cpu().to("cuda", torch.float16)):
+        a, b = cast(copy.deepcopy(lin)), cast(copy.deepcopy(experts))
+        for name in ("w_q", "w_scale"):
+            t, u = getattr(a, name), getattr(lin, name)
+            assert t.dtype == u.dtype and t.is_cuda and torch.equal(t.view(torch.uint8), u.view(torch.uint8))
+        assert torch.equal(a(x), plain + a.bias.to(torch.bfloat16)) and a(x).dtype == torch.bfloat16
+        assert torch.equal(b(z, ids, weights), want)
+    assert list(lin.state_dict()) == ["w_q", "w_scale", "bias"] and list(experts.half().state_dict()) == ["gate_up", "gate_up_scale", "down", "down_scale"]
