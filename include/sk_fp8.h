@@ -82,7 +82,8 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
  *   y_e(x) = W_down[e] q( SiLU(gate) * up ),   [gate; up] = W_gate_up[e] q(x),   q the quantiser above,
  *   out[t] = cast( sum_j weights[t, j] * y_{expert of (t, j)}(x[t]) ),   choices with rows outside [0, T * k) count nothing.
  * gate_up: 2 * experts matrices [inter, hidden] (an expert's gate, then its up; `experts` there counts matrices), down: experts
- * matrices [hidden, inter].  y is rounded to out_dtype before it is summed.  x_type: fp16 or bf16 or fp32. */
+ * matrices [hidden, inter].  y is rounded to out_dtype before it is summed.  x_type: fp16 or bf16 or fp32.  rows and offsets are those of
+ * one routing: a place that lies in no group has no result.  The workspace is 256-byte aligned. */
 int64_t sk_fp8_experts_workspace_bytes(int64_t T, int64_t k, int64_t hidden, int64_t inter, int scale_type);
 int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x, const int32_t* rows, const float* weights,
                    const int32_t* offsets, const sk_fp8_weight* gate_up, const sk_fp8_weight* down, int scale_type, void* out,
@@ -105,7 +106,7 @@ int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int sc
 typedef enum sk_fp8_option {
   SK_FP8_OPT_ROW_TILE = 1,          /* rows per tile of the kernel for few rows: 16 / 32 (16 where there is no 32) */
   SK_FP8_OPT_SPLIT_K = 2,           /* CTAs that share the K range of a tile (products of one group) */
-  SK_FP8_OPT_WAIT_LIMIT_CYCLES = 3, /* as SK_OPT_WAIT_LIMIT_CYCLES */
+  SK_FP8_OPT_WAIT_LIMIT_CYCLES = 3, /* as SK_OPT_WAIT_LIMIT_CYCLES, 10^6 at least */
   SK_FP8_OPT_TEST_SKIP_COPY = 4,    /* as SK_OPT_TEST_SKIP_COPY */
   SK_FP8_OPT_KERNEL = 5             /* sk_fp8_kernel; with 32-bit scales 3 means 2 */
 } sk_fp8_option;

@@ -162,7 +162,7 @@ fp8_prepare_weight_kernel(const void* w, long long ld_w, long long matrix, int N
     uint32_t code = e4m3x2(f[i][0] * inv, f[i][1] * inv) | (e4m3x2(f[i][2] * inv, f[i][3] * inv) << 16);
     if (bad) code = 0x7f7f7f7fu;
     uint8_t* dst = q + out + n * ld_q + col;
-    if (col + 4 <= K && (ld_q & 3) == 0) {
+    if (col + 4 <= K) {                             // (ld_q is a multiple of 16)
       *reinterpret_cast<uint32_t*>(dst) = code;
     } else {
       for (int j = 0; j < 4 && col + j < K; ++j) dst[j] = static_cast<uint8_t>(code >> (8 * j));

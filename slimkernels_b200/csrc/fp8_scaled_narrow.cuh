@@ -4,7 +4,8 @@
 // With few rows a product is a stream of weights out of HBM.  A K block is 16 KiB of weights and TOK x 128 B of activations, and all
 // that happens to it is a copy, four MMAs and a commit: what the kernel for 32-bit scales does per K block in its epilogue -- 700
 // cycles for one CTA, which held a projection of 4096 features and 16 rows to 44 GB/s per CTA -- is gone, and the stream is as fast as the ring
-// is deep: 16 x 18944 x K, a tile per SM, takes 3.4 us and then 6.2 TB/s.  (One SM draws 80 GB/s at most.)  The ring takes what shared memory there is: where a call has no more CTAs than SMs, all of it for one CTA, else half.
+// is deep: 16 x 18944 x K, a tile per SM, takes 3.4 us and then 6.2 TB/s.  (One SM draws 80 GB/s at most.)  The ring takes what shared
+// memory there is: where a call has no more CTAs than SMs, all of it for one CTA, else half.
 //
 // A tile's K range can be split over a cluster: every CTA pushes its sums into the CTA that owns the row (remote stores), one cluster
 // barrier, then the owner adds them in rank order, so the result does not depend on timing.
@@ -22,14 +23,11 @@ struct Fp8ScaledNarrowTraits {
   static constexpr int kStageBytes = kW * kFp8TileBytes + TOK * kFp8Block;
   static constexpr int kMaxStages = 12;
   static constexpr int kSlots = 4;
-  static constexpr int kXCols = (TOK + 31) / 32;    // columns of X's scales per slot; W's are 4 per weight tile
-  static constexpr int kSlotCols = kW * 4 + (kXCols + 3) / 4 * 4;
+  static constexpr int kSlotCols = kW * 4 + 4;      // 4 columns of scales per weight tile, and 4 for X (rows past 32 are not there)
   static constexpr int kSums = 2;                   // accumulator sets: the next tile's MMAs run while one is read
   static constexpr int kScaleCol0 = kSums * kW * TOK;
-  static constexpr int kNeedCols = kScaleCol0 + kSlots * kSlotCols;
-  static constexpr int kTmemCols = kNeedCols <= 128 ? 128 : kNeedCols <= 256 ? 256 : 512;
-  static constexpr int kCtas = kTmemCols <= 256 && kW * TOK <= 64 ? 2 : 1;      // per SM at most
-  static_assert(kNeedCols <= 512, "tensor memory");
+  static constexpr int kTmemCols = 128;
+  static_assert(TOK <= 32 && kScaleCol0 + kSlots * kSlotCols <= kTmemCols, "tensor memory");
   // behind the ring (whose depth is the launch's): barriers, then the reduction buffer or the group table
   static constexpr int kNumBars = 2 * kMaxStages + 2 * kSlots + 2 * kSums + 1;
   static constexpr int kOffAmax = (kNumBars * 8 + 16 + 15) / 16 * 16;           // SILU: [4 warps][TOK]
@@ -42,7 +40,7 @@ struct Fp8ScaledNarrowTraits {
 };
 
 template <int TOK, bool SILU>
-__global__ void __launch_bounds__(320, (Fp8ScaledNarrowTraits<TOK, SILU>::kCtas))
+__global__ void __launch_bounds__(320, 2)
 fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Fp8Params p) {
   using T = Fp8ScaledNarrowTraits<TOK, SILU>;
   constexpr int kW = T::kW;
@@ -199,7 +197,7 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     }
     __syncwarp();
   } else if (warp >= 4) {
-    // ------------------------------------------------------------ scales: lane l holds those of rows l, l + 32, ... of X; W's tile has one
+    // ------------------------------------------------------------ scales: lane l holds that of row l of X; W's tile has one
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + T::kScaleCol0;
     int slot = 0;
     uint32_t phase = 1;
@@ -210,13 +208,9 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
       const long long ws0 = (t.expert * p.scale_rows + t.n) * p.k_blocks;
       // groups of four are counted from this CTA's first block, which need not lie on a multiple of four
       const bool whole_w = p.w_scale_groups && (kb_begin & 3) == 0, whole_x = p.x_scale_groups && (kb_begin & 3) == 0;
-      uint32_t x[T::kXCols], w[kW];
+      uint32_t x, w[kW];
       auto fetch = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < T::kXCols; ++i) {
-          const int row = lane + 32 * i;
-          x[i] = load_exponents4(p.x_scale, static_cast<long long>(t.row0 + (row < t.rows ? row : 0)) * p.xs_row + kb * p.xs_blk, p.xs_blk, kb_end - kb, whole_x);
-        }
+        x = load_exponents4(p.x_scale, static_cast<long long>(t.row0 + (lane < t.rows ? lane : 0)) * p.xs_row + kb * p.xs_blk, p.xs_blk, kb_end - kb, whole_x);
 #pragma unroll
         for (int i = 0; i < kW; ++i) w[i] = load_exponents4(p.w_scale, ws0 + static_cast<long long>(i * p.up_block0) * p.k_blocks + kb, 1, kb_end - kb, whole_w);
       };
@@ -232,9 +226,7 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
           const uint32_t sa[4] = {w[i], w[i], w[i], w[i]};
           tmem_st_32x4(at + 4 * i, sa);
         }
-        uint32_t sb[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sb[i] = x[i < T::kXCols ? i : 0];
+        const uint32_t sb[4] = {x, x, x, x};
         tmem_st_32x4(at + 4 * kW, sb);
         tmem_st_wait();
         tcgen05_fence_before_sync();
@@ -255,19 +247,16 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     grid_dep_wait();
     for (int tile = tile0; tile < total && ok; tile += step) {
       const Fp8Tile t = fp8_tile_at<TOK>(tile, groups, p);
-      constexpr int kChunk = TOK < 32 ? TOK : 32;
-      uint32_t v[kW][TOK / kChunk][kChunk];
+      uint32_t v[kW][TOK];
       ok = wait_bounded_relaxed(bar_sum + 8 * set, phase, ctx, kStEpilogueAccFull, 20);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tcgen05_fence_after_sync();
 #pragma unroll
-        for (int w = 0; w < kW; ++w)
-#pragma unroll
-          for (int c = 0; c < TOK / kChunk; ++c) {
-            const uint32_t at = t_lane + (set * kW + w) * TOK + c * kChunk;
-            if constexpr (kChunk == 32) tmem_ld_32x32(at, v[w][c]); else tmem_ld_32x16(at, v[w][c]);
-          }
+        for (int w = 0; w < kW; ++w) {
+          const uint32_t at = t_lane + (set * kW + w) * TOK;
+          if constexpr (TOK == 32) tmem_ld_32x32(at, v[w]); else tmem_ld_32x16(at, v[w]);
+        }
         tmem_ld_wait();
         tcgen05_fence_before_sync();
         __syncwarp();
@@ -278,7 +267,7 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
       if constexpr (SILU) ok = named_barrier_all(1, 128, ok);
       if (!ok) break;
       const int n = t.n * 128 + feature;
-      auto sum = [&](int w, int j) { return __uint_as_float(v[w][j / kChunk][j % kChunk]); };
+      auto sum = [&](int w, int j) { return __uint_as_float(v[w][j]); };
       if constexpr (SILU) {
         // a feature past the end counts as zero in its block's maximum
         float* part = reinterpret_cast<float*>(behind + T::kOffAmax);
@@ -286,7 +275,7 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         float h[TOK];
 #pragma unroll
         for (int j = 0; j < TOK; ++j) {
-          if (j >= t.rows) break;                   // (groups of a few rows in a tile of 32: a third of the kernel)
+          if (j >= t.rows) break;                   // (most groups have a few rows)
           h[j] = live ? silu_times(sum(0, j), sum(1, j)) : 0.f;
           uint32_t a = __float_as_uint(h[j]) & 0x7fffffffu;      // (ordered like the values; NaN above all)
           a = __reduce_max_sync(0xffffffffu, a);

@@ -4,15 +4,16 @@
 // block's), so the epilogue is one FFMA per value; with features on the lanes every column has its own scale, a load more per four.  256
 // columns instead of 128 halve the bytes of X that a MMA reads again.
 //
-// What bounds it: 4096 x 8192 x 8192 takes 309 us (1780 TFLOP/s), about 1130 cycles a K block.  The MMAs are 512 of them, shared memory (48 KiB
-// in by TMA, 48 KiB out to the tensor core, 128 B a cycle) makes that 768, and measured without the epilogue's arithmetic a block takes 790 to 860.
-// The 128 FFMAs of each epilogue thread add their issue time to that, wherever they stand: sixteen epilogue warps (1290), loading the next
-// block's columns ahead (1280) and a second issuer (1120) gain nothing.  With 8-bit scales none of this is needed (fp8_scaled.cuh).
 // Two accumulators of 256 columns fill the tensor memory: the MMAs of one K block run while eight warps drain the other.
 //   producer   one thread: TMA of 128 x 128 B of X and two boxes of 128 x 128 B of W per K block, four stages of 48 KiB
 //   issuer     one thread: four MMAs of 128 x 256 x 32 per K block and one commit, which serves the producer and the epilogue
 //   epilogue   two warpgroups, each a row per thread and 128 of the 256 columns, fp32 sums in registers
 // The CTAs stay and walk the tiles; the operands of the next tile are on their way while a tile is written.
+//
+// What bounds it: 4096 x 8192 x 8192 takes 309 us (1780 TFLOP/s), about 1130 cycles a K block.  The MMAs are 512 of them, shared memory (48 KiB
+// in by TMA, 48 KiB out to the tensor core, 128 B a cycle) makes that 768, and measured without the epilogue's arithmetic a block takes 790 to 860.
+// The 128 FFMAs of each epilogue thread add their issue time to that, wherever they stand: sixteen epilogue warps (1290), loading the next
+// block's columns ahead (1280) and a second issuer (1120) gain nothing.  With 8-bit scales none of this is needed (fp8_scaled.cuh).
 //
 // SILU: the columns are 128 gate features and the 128 up features beside them, and a thread takes 64 of either, so that SiLU(gate) * up
 // and its quantisation (one block of the next product per row) stay in registers but for the two halves' maxima.
@@ -23,7 +24,6 @@ namespace sk {
 
 template <bool SILU>
 struct Fp8WideTraits {
-  static constexpr int kRows = 128;
   static constexpr int kStages = 4, kBufs = 2;
   static constexpr int kRing = kStages;             // "block done" barriers: R >= S and R >= B, as in the narrow kernel
   static constexpr int kStageBytes = 3 * kFp8TileBytes;

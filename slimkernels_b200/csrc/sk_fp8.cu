@@ -100,7 +100,8 @@ int64_t scale_bytes(int scale_type) { return scale_type == SK_SCALE_E8M0 ? 1 : 4
 
 // dependent: programmatic dependent launch.  Every kernel here but the weight preparation waits (griddepcontrol.wait) before it reads or
 // writes global memory, so its set-up may run under the tail of whatever is in front of it; that saves 1 to 2 us a launch between
-// this library's kernels, which let their followers start early.
+// this library's kernels, which let their followers start early.  (A follower may hold tensor memory while it waits.  It cannot take any that the
+// kernel in front still needs: every kernel here takes at most half of an SM's columns with half of its shared memory, or all with most of it.)
 struct LaunchConfig {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -234,7 +235,7 @@ int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params
   auto kern = fp8_scaled_narrow_kernel<TOK, SILU>;
   constexpr int kSm = 233472, kCta = 232448;        // shared memory of an SM (1 KiB per CTA goes to the system) and of a CTA
   const int fixed = T::fixed_bytes(p.split, p.experts);
-  int ctas = T::kCtas == 2 && tiles * p.split > dev.sms ? 2 : 1;
+  int ctas = tiles * p.split > dev.sms ? 2 : 1;
   if ((kSm / ctas - 1024 - fixed) / T::kStageBytes < 3) ctas = 1;
   p.stages = std::min(T::kMaxStages, ((ctas == 1 ? kCta : kSm / 2 - 1024) - fixed) / T::kStageBytes);
   static_assert((kCta - T::fixed_bytes(SILU ? 1 : 8, 1)) / T::kStageBytes >= 3 && (kCta - T::fixed_bytes(1, kFp8MaxExperts)) / T::kStageBytes >= 3, "room for a ring");
@@ -636,7 +637,8 @@ int sk_fp8_set_option(int key, int64_t value) {
       if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_WAIT_LIMIT_CYCLES:
-      if (value != 0 && value < 1000) return SK_ERR_BAD_ARGUMENT;
+      // (a wait is not given up before every copy in flight has long landed: a producer that is done does not look after its last ones)
+      if (value != 0 && value < 1000000) return SK_ERR_BAD_ARGUMENT;
       break;
     case SK_FP8_OPT_KERNEL:
       if (value > SK_FP8_KERNEL_PAIR) return SK_ERR_BAD_ARGUMENT;

@@ -149,10 +149,24 @@ def test_router_and_experts_refuse_bad_arguments(built_libs):
 def test_options_are_checked(built_libs):
     from slimkernels_b200 import capi
     lib = capi.load()
-    for key, value in [(1, 48), (1, -1), (2, 3), (3, 10), (0, 0), (99, 0), (5, 4), (1, 64)]:
+    for key, value in [(1, 48), (1, -1), (2, 3), (3, 10), (3, 999_999), (0, 0), (99, 0), (5, 4), (1, 64)]:
         assert lib.sk_fp8_set_option(key, value) == capi.SK_ERR_BAD_ARGUMENT, (key, value)
     for key in (1, 2, 3, 4, 5):
         assert lib.sk_fp8_set_option(key, 0) == capi.SK_OK
+
+
+def test_module_casts_leave_codes_and_scales_alone():
+    import slimkernels_b200.torch as sk
+    codes = torch.arange(126, dtype=torch.uint8).repeat(64)[:4096].view(32, 128).view(torch.float8_e4m3fn)
+    scale = torch.tensor([[254]], dtype=torch.uint8).view(torch.float8_e8m0fnu)             # (beyond fp16's range)
+    m = sk.FP8Linear(codes, scale, 120, torch.ones(32), torch.float16)
+    for cast in (m.half, m.double, lambda: m.to(torch.bfloat16), lambda: m.to("cpu", torch.float16)):
+        assert cast() is m
+        assert m.w_q.dtype == codes.dtype and torch.equal(m.w_q.view(torch.uint8), codes.view(torch.uint8))
+        assert m.w_scale.dtype == scale.dtype and torch.equal(m.w_scale.view(torch.uint8), scale.view(torch.uint8))
+    assert m.bias.dtype == torch.float16
+    assert m.to("meta").w_q.is_meta and m.w_q.dtype == codes.dtype
+    assert list(m.state_dict()) == ["w_q", "w_scale", "bias"]
 
 
 def test_torch_ops_refuse_host_tensors(built_libs):
