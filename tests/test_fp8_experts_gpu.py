@@ -282,6 +282,91 @@ def test_captured_layers_follow_their_inputs():
         assert torch.equal(y, run())
 
 
+def test_one_expert_twice_and_very_many_choices():
+    T, E, hidden, inter = 9, 3, 128, 144
+    g, gu, dn = _layers(E, hidden, inter, E8M0, 11)
+    x = F.random_rows(g, T, hidden, torch.bfloat16)
+    for k in (2, 40):                                       # (more choices than there are experts, and than a warp has lanes)
+        ids = torch.randint(0, E, (T, k), generator=g, device="cuda")
+        ids[:, 1] = ids[:, 0]
+        weights = torch.rand(T, k, generator=g, device="cuda")
+        rows, offsets = sk.group_by_expert(ids, E)
+        y = sk.fp8_experts(x, sk.Routing(None, weights, rows, offsets), *gu, *dn)
+        _check_experts(x, rows, weights, offsets, gu, dn, y)
+
+
+def test_as_many_experts_as_there_may_be():
+    T, E, hidden, inter = 70, 1024, 128, 128
+    for scales in (E8M0, F32):
+        g, gu, dn = _layers(E, hidden, inter, scales, 12)
+        x = F.random_rows(g, T, hidden, torch.float16)
+        routing = sk.route_tokens(torch.randn(T, E, generator=g, device="cuda"), 32)
+        _check_experts(x, routing.rows, routing.weights, routing.offsets, gu, dn, sk.fp8_experts(x, routing, *gu, *dn))
+
+
+def test_all_tokens_to_one_expert():
+    T, E, hidden, inter = 600, 64, 256, 128
+    for scales in (E8M0, F32):
+        g, gu, dn = _layers(E, hidden, inter, scales, 13)
+        x = F.random_rows(g, T, hidden, torch.bfloat16)
+        logits = torch.full((T, E), float("-inf"), device="cuda")
+        logits[:, 63] = torch.randn(T, generator=g, device="cuda")
+        routing = sk.route_tokens(logits, 1)
+        assert routing.offsets.tolist() == [0] * 64 + [T]
+        _check_experts(x, routing.rows, routing.weights, routing.offsets, gu, dn, sk.fp8_experts(x, routing, *gu, *dn))
+
+
+def test_layers_on_two_streams_at_once():
+    T, E, k, hidden, inter = 40, 8, 2, 512, 256
+    sets = []
+    for seed in (1, 2):
+        g, gu, dn = _layers(E, hidden, inter, E8M0, seed)
+        sets.append((F.random_rows(g, T, hidden, torch.bfloat16), torch.randn(T, E, generator=g, device="cuda"), gu, dn))
+    run = lambda x, logits, gu, dn: sk.fp8_experts(x, sk.route_tokens(logits, k), *gu, *dn)      # noqa: E731
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in (0, 1) for y in got[i])
+
+
+def test_two_graphs_that_share_their_memory():
+    T, E, k, hidden, inter = 24, 8, 2, 256, 128
+    g, gu, dn = _layers(E, hidden, inter, E8M0, 14)
+    xs = [F.random_rows(g, n, hidden, torch.bfloat16) for n in (T, T + 70)]
+    logits = [torch.randn(len(x), E, generator=g, device="cuda") for x in xs]
+    run = lambda i: sk.fp8_experts(xs[i], sk.route_tokens(logits[i], k), *gu, *dn)      # noqa: E731
+    want = [run(i).clone() for i in (0, 1)]
+    pool, graphs, out = torch.cuda.graph_pool_handle(), [], []
+    for i in (0, 1):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], pool=pool):
+            out.append(run(i))
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        assert torch.equal(out[i], want[i])
+
+
+def test_places_past_32_bits():
+    """More than 2^31 codes and results in the layers' workspace: the last tokens against the definition."""
+    T, E, k, hidden, inter = 66000, 4, 8, 4096 + 16, 128
+    g, gu, dn = _layers(E, hidden, inter, E8M0, 15)
+    x = F.random_rows(g, T, hidden, torch.bfloat16)
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    weights = torch.rand(T, k, generator=g, device="cuda")
+    rows, offsets = sk.group_by_expert(ids, E)
+    assert T * k * hidden > 2 ** 31 and offsets.tolist() == [0, *torch.bincount(ids.flatten(), minlength=E).cumsum(0).tolist()]
+    y = sk.fp8_experts(x, sk.Routing(ids, weights, rows, offsets), *gu, *dn)
+    for part in (slice(0, 20), slice(T - 40, T)):
+        r, o = sk.group_by_expert(ids[part].contiguous(), E)
+        _check_experts(x[part], r, weights[part], o, gu, dn, y[part])
+
+
 def test_expert_layer_refusals():
     g, gu, dn = _layers(4, 128, 256, E8M0, 1)
     x = torch.randn(6, 128, device="cuda")

@@ -427,6 +427,51 @@ def test_nan_stays_in_its_group():
     assert bool(nan[10].all()) and bool(nan[20:].all()) and not bool(nan[:10].any()) and not bool(nan[11:20].any())
 
 
+# --------------------------------------------------------------------------------------------------- offsets past 32 bits
+@pytest.mark.parametrize("M,N,K", [(264000, 128, 8192), (264000, 8200, 128)])
+@pytest.mark.parametrize("scales", [E8M0, F32])
+def test_linear_layers_past_32_bits(M, N, K, scales):
+    """More than 2^31 activations, or results."""
+    g = F.generator(N)
+    w = sk.prepare_weight_fp8(torch.randn(N, K, generator=g, device="cuda"), scales)
+    x = torch.randn(M, K, generator=g, device="cuda", dtype=torch.bfloat16)
+    y = sk.fp8_linear(x, *w)
+    for part in (slice(0, 20), slice(M - 70, M)):
+        exact, tol = F.product_tolerance(F.quantised_values(x[part]), F.weight_values(*w), torch.bfloat16)
+        F.assert_within(y[part], exact, tol)
+
+
+@pytest.mark.parametrize("kernel", [capi.FP8_FEW, capi.FP8_MANY, capi.FP8_PAIR])
+@pytest.mark.parametrize("scales", [E8M0, F32])
+def test_weights_past_32_bits(kernel, scales, forced):
+    E, N, K = 33, 8192, 8192
+    g = F.generator(8)
+    assert E * N * K > 2 ** 31
+    w_q = (torch.randint(0, 256, (E, N, K), generator=g, device="cuda", dtype=torch.uint8) & 0xbe).view(torch.float8_e4m3fn)
+    w_s = F.pow2(torch.randint(-4, 5, (E, N // 128, K // 128), generator=g, device="cuda")).float().to(scales)
+    off = [0, 3] + [3] * (E - 3) + [5, 25]
+    x = sk.quantize_fp8(F.random_rows(g, 25, K, torch.bfloat16), scales)
+    forced(kernel=kernel)
+    y = sk.fp8_grouped_gemm(*x, w_q, w_s, torch.tensor(off, dtype=torch.int32, device="cuda"))
+    for e in (0, E - 2, E - 1):
+        part = slice(off[e], off[e + 1])
+        exact, tol = F.product_tolerance(F.row_values(x[0][part], x[1][part]), F.weight_values(w_q[e], w_s[e]), torch.bfloat16)
+        F.assert_within(y[part], exact, tol)
+
+
+def test_rows_far_apart():
+    """A column slice of a matrix whose rows lie 2^29 bytes apart: pitches in 64 bits."""
+    base = torch.zeros(6, 2 ** 29, dtype=torch.uint8, device="cuda")
+    x_q, x_s = sk.quantize_fp8(torch.randn(6, 256, device="cuda", generator=F.generator(9)))
+    far = base[:, 4096:4096 + 256].view(torch.float8_e4m3fn)
+    far.view(torch.uint8).copy_(x_q.view(torch.uint8))
+    w = sk.prepare_weight_fp8(torch.randn(160, 256, device="cuda", generator=F.generator(10)))
+    out = base[:, 2 ** 28:2 ** 28 + 320].view(torch.bfloat16)
+    want = sk.fp8_gemm(x_q, x_s, *w)
+    sk.fp8_gemm(far, x_s, *w, out=out)
+    assert torch.equal(out, want) and torch.equal(sk.quantize_fp8(out)[0].view(torch.uint8), sk.quantize_fp8(want)[0].view(torch.uint8))
+
+
 # -------------------------------------------------------------------------------------------- streams, graphs, failure
 def test_captured_products_follow_their_inputs():
     g = F.generator(6)
