@@ -10,10 +10,13 @@
 //   epilogue   two warpgroups, each a row per thread and 128 of the 256 columns, fp32 sums in registers
 // The CTAs stay and walk the tiles; the operands of the next tile are on their way while a tile is written.
 //
-// What bounds it: 4096 x 8192 x 8192 takes 309 us (1780 TFLOP/s), about 1130 cycles a K block.  The MMAs are 512 of them, shared memory (48 KiB
-// in by TMA, 48 KiB out to the tensor core, 128 B a cycle) makes that 768, and measured without the epilogue's arithmetic a block takes 790 to 860.
-// The 128 FFMAs of each epilogue thread add their issue time to that, wherever they stand: sixteen epilogue warps (1290), loading the next
-// block's columns ahead (1280) and a second issuer (1120) gain nothing.  With 8-bit scales none of this is needed (fp8_scaled.cuh).
+// What bounds it: 4096 x 8192 x 8192 takes 309 us (1780 TFLOP/s; 260 before the power settles), about 1050 cycles a K block.  The MMAs are 512 of
+// them, shared memory (48 KiB in by TMA, 48 KiB out to the tensor core, 128 B a cycle) makes that 768.  The 128 FFMAs of each epilogue thread add
+// 200 to 250 wherever they stand, with operands of zeros (no power limit) as well: 223 us, 180 without them, 176 without the loads of the sums, too.
+// Measured and not kept: pairs of CTAs (shared memory then takes 512: 253 against 257 us, ragged groups up to 40 % slower), accumulators in four halves
+// with barriers of their own (2 % faster here, up to 13 % slower with 16 K blocks), two warps that multiply the scales, results through shared memory,
+// sixteen epilogue warps, the next block's columns loaded ahead, a second issuer (nothing), two FFMAs an instruction (spills).  With 8-bit
+// scales none of this is needed (fp8_scaled.cuh).
 //
 // SILU: the columns are 128 gate features and the 128 up features beside them, and a thread takes 64 of either, so that SiLU(gate) * up
 // and its quantisation (one block of the next product per row) stay in registers but for the two halves' maxima.
