@@ -1,6 +1,7 @@
 // The FP8 ops of namespace `slimkernels` (slimkernels_b200/torch/fp8.py): tensors into the C ABI of include/sk_fp8.h.  No kernels
 // live here.  Inference only, like the W2A8 ops: nothing is recorded for a backward pass.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
 #include <torch/library.h>
@@ -19,6 +20,11 @@ void check(int rc, const char* what) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// at::empty on like's device without a turn through the dispatcher (0.4 us each; a router call makes four).
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(size, type, like.device(), c10::nullopt));
+}
 
 int float_type(const at::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -132,8 +138,8 @@ int one_scale_type(const at::Tensor& a, const at::Tensor& b) {
 // Empty codes [M, K] with rows on 16 bytes, and their scales in the order the products read fastest.
 std::tuple<at::Tensor, at::Tensor> empty_rows(const at::Tensor& like, int64_t M, int64_t K, at::ScalarType scales) {
   const int64_t kb = ceil_div(K, 128);
-  at::Tensor q = at::empty({M, round_up(K, 16)}, like.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, K);
-  at::Tensor s = at::empty({M, round_up(kb, 4)}, like.options().dtype(scales)).narrow(1, 0, kb);
+  at::Tensor q = fresh({M, round_up(K, 16)}, at::kFloat8_e4m3fn, like).narrow(1, 0, K);
+  at::Tensor s = fresh({M, round_up(kb, 4)}, scales, like).narrow(1, 0, kb);
   return {q, s};
 }
 
@@ -200,7 +206,7 @@ void fp8_gemm_out(const at::Tensor& x_q, const at::Tensor& x_scale, const at::Te
 at::Tensor fp8_gemm(const at::Tensor& x_q, const at::Tensor& x_scale, const at::Tensor& w_q, const at::Tensor& w_scale, at::ScalarType out_dtype) {
   out_type(out_dtype);
   TORCH_CHECK(x_q.dim() == 2 && w_q.dim() == 2, "x_q must have shape [M, K] and w_q [N, K]");
-  at::Tensor out = at::empty({x_q.size(0), w_q.size(0)}, x_q.options().dtype(out_dtype));
+  at::Tensor out = fresh({x_q.size(0), w_q.size(0)}, out_dtype, x_q);
   fp8_gemm_out(x_q, x_scale, w_q, w_scale, out);
   return out;
 }
@@ -217,10 +223,10 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w_q, const at::Tens
   const at::ScalarType dt = default_out(x, out_dtype);
   const int ot = out_type(dt);
   c10::cuda::CUDAGuard guard(x2.device());
-  at::Tensor out = at::empty({M, w.N}, x2.options().dtype(dt));
+  at::Tensor out = fresh({M, w.N}, dt, x2);
   if (M > 0) {
     const int64_t bytes = sk_fp8_linear_workspace_bytes(M, w.K, st);
-    at::Tensor ws = at::empty({bytes}, x2.options().dtype(at::kByte));     // caching allocator: 512-byte aligned
+    at::Tensor ws = fresh({bytes}, at::kByte, x2);     // caching allocator: 512-byte aligned
     check(sk_fp8_linear(M, x2.data_ptr(), ft, pitch(x2), &w, st, out.data_ptr(), w.N, ot, ws.data_ptr(), bytes,
                         at::cuda::getCurrentCUDAStream().stream()),
           "fp8_linear");
@@ -257,7 +263,7 @@ at::Tensor fp8_grouped_gemm(const at::Tensor& x_q, const at::Tensor& x_scale, co
                             const at::Tensor& offsets, at::ScalarType out_dtype) {
   out_type(out_dtype);
   TORCH_CHECK(x_q.dim() == 2 && w_q.dim() == 3, "x_q must have shape [M, K] and w_q [experts, N, K]");
-  at::Tensor out = at::empty({x_q.size(0), w_q.size(1)}, x_q.options().dtype(out_dtype));
+  at::Tensor out = fresh({x_q.size(0), w_q.size(1)}, out_dtype, x_q);
   fp8_grouped_gemm_out(x_q, x_scale, w_q, w_scale, offsets, out);
   return out;
 }
@@ -269,11 +275,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_tokens(const at
   TORCH_CHECK(E >= 1 && E <= 1024 && k >= 1 && k <= std::min<int64_t>(E, 32), "1 <= k <= min(E, 32) and E <= 1024 are wanted, got k = ", k, ", E = ", E);
   const at::Tensor l = as_rows(logits, "logits");
   c10::cuda::CUDAGuard guard(l.device());
-  const auto ints = l.options().dtype(at::kInt);
-  at::Tensor ids = at::empty({T, k}, ints), weights = at::empty({T, k}, l.options().dtype(at::kFloat)), rows = at::empty({T, k}, ints);
-  at::Tensor offsets = at::empty({E + 1}, ints);
+  at::Tensor ids = fresh({T, k}, at::kInt, l), weights = fresh({T, k}, at::kFloat, l), rows = fresh({T, k}, at::kInt, l);
+  at::Tensor offsets = fresh({E + 1}, at::kInt, l);
   const int64_t bytes = sk_route_workspace_bytes(T, E);
-  at::Tensor ws = bytes > 0 ? at::empty({bytes}, l.options().dtype(at::kByte)) : offsets;
+  at::Tensor ws = bytes > 0 ? fresh({bytes}, at::kByte, l) : offsets;
   // (an empty tensor has no address; nothing is read or written through these when T = 0)
   void* some = offsets.data_ptr();
   check(sk_route_tokens(T ? l.data_ptr() : some, ft, T ? pitch(l) : E, T, E, k, renormalize, static_cast<int*>(T ? ids.data_ptr() : some),
@@ -291,9 +296,9 @@ std::tuple<at::Tensor, at::Tensor> group_by_expert(const at::Tensor& ids_in, int
   // (64-bit ids are cut to the range that 32 bits hold, so that none wraps into a valid one)
   const at::Tensor ids = (ids_in.scalar_type() == at::kLong ? ids_in.clamp(-1, E).to(at::kInt) : ids_in).contiguous();
   const int64_t T = ids.size(0), k = ids.size(1);
-  at::Tensor rows = at::empty({T, k}, ids.options()), offsets = at::empty({E + 1}, ids.options());
+  at::Tensor rows = fresh({T, k}, at::kInt, ids), offsets = fresh({E + 1}, at::kInt, ids);
   const int64_t bytes = sk_route_workspace_bytes(T, E);
-  at::Tensor ws = bytes > 0 ? at::empty({bytes}, ids.options().dtype(at::kByte)) : offsets;
+  at::Tensor ws = bytes > 0 ? fresh({bytes}, at::kByte, ids) : offsets;
   void* some = offsets.data_ptr();
   check(sk_group_by_expert(static_cast<const int*>(T ? ids.data_ptr() : some), T, k, E, static_cast<int*>(T ? rows.data_ptr() : some),
                            offsets.data_ptr<int>(), ws.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()),
@@ -325,10 +330,10 @@ at::Tensor fp8_experts(const at::Tensor& x, const at::Tensor& rows, const at::Te
   const at::ScalarType dt = default_out(x, out_dtype);
   const int ot = out_type(dt);
   c10::cuda::CUDAGuard guard(x2.device());
-  at::Tensor out = at::empty({T, gu.K}, x2.options().dtype(dt));
+  at::Tensor out = fresh({T, gu.K}, dt, x2);
   if (T > 0) {
     const int64_t bytes = sk_fp8_experts_workspace_bytes(T, k, gu.K, gu.N, st);
-    at::Tensor ws = at::empty({bytes}, x2.options().dtype(at::kByte));
+    at::Tensor ws = fresh({bytes}, at::kByte, x2);
     check(sk_fp8_experts(T, k, x2.data_ptr(), ft, pitch(x2), rows.data_ptr<int>(), weights.data_ptr<float>(), offsets.data_ptr<int>(), &gu, &dn, st,
                          out.data_ptr(), gu.K, ot, ws.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()),
           "fp8_experts");
