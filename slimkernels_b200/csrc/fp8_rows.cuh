@@ -215,10 +215,11 @@ fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const flo
 // ---------------------------------------------------------------- router
 // A CTA takes a run of tokens, a warp a run of those; everything is in the order of the choices t * k + j, so the places are those
 // of a stable sort by expert and the same in every run.
-//   pass 1  (TOPK: the k largest logits of each token and their weights) and how many choices each expert got from this CTA
-//   pass 2  (after pass 1 of all CTAs) the experts' first rows, and the place of each choice
-// With one CTA both are one launch.  Latency bounds all of it (8192 tokens of 256 logits are 4 MB): 32 warps to a CTA, a token's logits
-// loaded while the one before it is worked on.
+//   pass 1  (TOPK: the k largest logits of each token and their weights,) how many choices each expert got from this CTA, and the place of each
+//           choice among these
+//   pass 2  (after pass 1 of all CTAs) the experts' first rows, added to the places
+// With one CTA both are one launch.  Issue slots and latency bound all of it (8192 tokens of 256 logits are 4 MB): 32 warps to a CTA, a token's
+// logits loaded while the one before it is worked on, as few instructions per choice as can be.
 constexpr int kRouteWarps = 32;
 struct RouteParams {
   const void* logits;                   // [T, ld]
@@ -246,10 +247,14 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t o) {
 // One token: lane holds the logits of experts lane, lane + 32, ...; the choice of a round is the largest left, the lowest expert among equals.
 // A logit of 16 bits and its expert fit one word, so that a round is one reduction and no two words are equal:
 //   bits that order like the logits | 0xffff - expert
-// 32-bit logits take a second reduction where several lanes hold the largest.  Only the lane that held it looks through its logits again.
+// A lane sorts its words first; the lane that held a round's largest moves on to its next.  (Looking through its words again instead: 12.1
+// against 9.7 us for 64 tokens of 256 experts.)
+// 32-bit logits take a second reduction where several lanes hold the largest.  The lane that held it looks through its logits again, as it does among
+// more than 512 experts.
 template <int TYPE, int PER>
 struct TokenLogits {
   static constexpr bool kWord = TYPE != 2;
+  static constexpr bool kSorted = kWord && PER <= 16;         // (32 words take more registers than a thread has)
   uint32_t key[PER];                    // 0: none (below -infinity's)
 
   static __device__ __forceinline__ uint32_t order16(uint32_t b) {
@@ -257,6 +262,22 @@ struct TokenLogits {
     if (nan) return 0xffffu;
     if (b == 0x8000u) b = 0;
     return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+  }
+  // Batcher's odd-even merge sort, the largest first.
+  __device__ __forceinline__ void sort() {
+#pragma unroll
+    for (int p = 1; p < PER; p *= 2)
+#pragma unroll
+      for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+        for (int j = d % p; j + d < PER; j += 2 * d)
+#pragma unroll
+          for (int i = 0; i < d; ++i)
+            if (i + j + d < PER && (i + j) / (2 * p) == (i + j + d) / (2 * p)) {
+              const uint32_t a = key[i + j], b = key[i + j + d];
+              key[i + j] = max(a, b);
+              key[i + j + d] = min(a, b);
+            }
   }
   static __device__ __forceinline__ float value16(uint32_t o) {
     if (o == 0xffffu) return __uint_as_float(0x7fc00000u);
@@ -295,57 +316,80 @@ struct TokenLogits {
 
   __device__ __forceinline__ void choose(const RouteParams& p, long long t, int lane) {
     order(p, lane);
-    uint32_t best = 0;
-    int at = 0;
-    auto look = [&]() {                 // the lane's own largest; 0: none left
-      best = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if constexpr (kWord) best = max(best, key[i]);
-        else if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
-      }
-    };
-    look();
-    float top = 0.f, sum = 0.f, mine = 0.f;
-    uint32_t first = 0;
+    uint32_t first, mine = 0;                         // the largest of all, and (lane j) choice j
     int my_id = 0;
-    for (int j = 0; j < p.k; ++j) {
-      const uint32_t winner = __reduce_max_sync(0xffffffffu, best);
-      int e;
-      if constexpr (kWord) {
-        e = static_cast<int>(0xffffu - (winner & 0xffffu));
-      } else {
-        const uint32_t holders = __ballot_sync(0xffffffffu, best == winner);
-        e = __shfl_sync(0xffffffffu, at, __ffs(holders) - 1);
-        if (holders & (holders - 1)) e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
+    float sum = 0.f;
+    const auto total = [&](uint32_t largest) {        // of the whole softmax, while all keys are there
+      const float top = value(largest);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (lane + 32 * i < p.E) sum += expf(value(key[i]) - top);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    };
+    if constexpr (kSorted) {
+      if (!p.renormalize) {
+        uint32_t most = key[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) most = max(most, key[i]);
+        total(__reduce_max_sync(0xffffffffu, most));
       }
-      if (j == 0) {
-        first = winner;
-        top = value(winner);
-        if (!p.renormalize) {           // the whole softmax's sum, while all keys are there
+      sort();
+      first = 0;
+      for (int j = 0; j < p.k; ++j) {
+        const uint32_t winner = __reduce_max_sync(0xffffffffu, key[0]);
+        if (key[0] == winner) {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) key[i] = i + 1 < PER ? key[i + 1] : 0;
+        }
+        if (j == 0) first = winner;
+        if (lane == j) mine = winner;
+      }
+      my_id = static_cast<int>(0xffffu - (mine & 0xffffu));
+    } else {
+      uint32_t best = 0;
+      int at = 0;
+      auto look = [&]() {               // the lane's own largest; 0: none left
+        best = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          if constexpr (kWord) best = max(best, key[i]);
+          else if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+        }
+      };
+      look();
+      first = 0;
+      for (int j = 0; j < p.k; ++j) {
+        const uint32_t winner = __reduce_max_sync(0xffffffffu, best);
+        int e;
+        if constexpr (kWord) {
+          e = static_cast<int>(0xffffu - (winner & 0xffffu));
+        } else {
+          const uint32_t holders = __ballot_sync(0xffffffffu, best == winner);
+          e = __shfl_sync(0xffffffffu, at, __ffs(holders) - 1);
+          if (holders & (holders - 1)) e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == winner ? static_cast<uint32_t>(at) : 0x7fffffffu));
+        }
+        if (j == 0) {
+          first = winner;
+          if (!p.renormalize) total(winner);
+        }
+        if ((e & 31) == lane) {
 #pragma unroll
           for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < p.E) sum += expf(value(key[i]) - top);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (kWord ? key[i] == winner : lane + 32 * i == e) key[i] = 0;
+          look();
         }
+        if (lane == j) { mine = winner; my_id = e; }
       }
-      if ((e & 31) == lane) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (kWord ? key[i] == winner : lane + 32 * i == e) key[i] = 0;
-        look();
-      }
-      if (lane == j) { mine = value(winner); my_id = e; }
     }
     // lane j holds choice j: its weight, and the sum of all in the order of the choices
-    mine = expf(mine - top);
+    const float w = expf(value(mine) - value(first));
     if (p.renormalize)
-      for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, mine, j);
+      for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, w, j);
     if (lane < p.k) {
       p.ids[t * p.k + lane] = my_id;
       // a token whose logits are all -infinity has no distribution: its weights are zero
-      p.weights[t * p.k + lane] = masked(first) ? 0.f : mine / sum;
+      p.weights[t * p.k + lane] = masked(first) ? 0.f : w / sum;
     }
   }
 };
@@ -371,9 +415,10 @@ __device__ __forceinline__ void route_count(const RouteParams& p, int* hist) {
     if (r.t0 < r.t1) now.load(p, r.t0, lane);
     for (int i = threadIdx.x; i < warps * p.E; i += blockDim.x) hist[i] = 0;
     for (long long t = r.t0; t < r.t1; ++t) {
-      if (t + 1 < r.t1) next.load(p, t + 1, lane);
+      if (PER <= 16 && t + 1 < r.t1) next.load(p, t + 1, lane);
       now.choose(p, t, lane);
-      now = next;
+      if (PER <= 16) now = next;
+      else if (t + 1 < r.t1) now.load(p, t + 1, lane);      // (no registers for two tokens' logits)
     }
     __syncwarp();
   } else {
@@ -448,8 +493,8 @@ __device__ __forceinline__ void scan_experts(int* total, int E) {
   __syncthreads();
 }
 
-// Shared memory: [warps][E] counts, [E + 1] totals, [E] first places of this CTA.
-__host__ __device__ constexpr int route_smem_bytes(int warps, int E) { return (warps * E + 2 * E + 1) * 4; }
+// Shared memory of pass 1: [warps][E] counts, [E + 1] first places.
+__host__ __device__ constexpr int route_smem_bytes(int warps, int E) { return (warps * E + E + 1) * 4; }
 
 template <int TYPE, int PER, bool TOPK, bool ONE_CTA>
 __global__ void __launch_bounds__(kRouteWarps * 32)
@@ -464,27 +509,31 @@ route_count_kernel(const RouteParams p) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int n = 0;
     for (int w = 0; w < warps; ++w) n += hist[w * p.E + e];
-    if constexpr (ONE_CTA) total[e] = n; else p.counts[static_cast<long long>(blockIdx.x) * p.E + e] = n;
+    if constexpr (!ONE_CTA) p.counts[static_cast<long long>(blockIdx.x) * p.E + e] = n;
+    total[e] = ONE_CTA ? n : 0;
   }
+  __syncthreads();
   if constexpr (ONE_CTA) {
-    __syncthreads();
     scan_experts(total, p.E);
     for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = total[e];
-    route_place(p, hist, total);
   }
+  route_place(p, hist, total);
 }
 
-__global__ void __launch_bounds__(kRouteWarps * 32)
-route_place_kernel(const RouteParams p) {
+// Adds the experts' first places, and what the CTAs in front chose, to the places.
+__global__ void __launch_bounds__(1024)
+route_shift_kernel(const RouteParams p) {
   extern __shared__ int route_smem[];
-  const int warps = blockDim.x >> 5;
-  int* hist = route_smem;
-  int* total = hist + warps * p.E;
-  int* base = total + p.E + 1;
+  int* total = route_smem;              // [E + 1]
+  int* base = total + p.E + 1;          // [E]
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) total[e] = base[e] = 0;
+  __syncthreads();
   grid_dep_wait();
   grid_dep_launch_dependents();
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) total[e] = base[e] = 0;
-  route_count<0, 1, false>(p, hist);                 // this CTA's counts by warp, again
+  const long long c0 = static_cast<long long>(blockIdx.x) * p.per_cta, c1 = min(static_cast<long long>(p.T), c0 + p.per_cta);
+  const long long i0 = c0 * p.k + threadIdx.x;      // (a thread's first place is on its way with the counts)
+  const bool on = i0 < c1 * p.k;
+  const int at0 = on ? ld_global_int(p.rows + i0) : -1, e0 = on ? ld_global_int(p.ids + i0) : 0;
   // the counts of all CTAs, and of those in front of this one: as many threads per expert as there are
   const int share = max(1, static_cast<int>(blockDim.x) / p.E), ctas = static_cast<int>(gridDim.x);
   for (int i = threadIdx.x; i < share * p.E; i += blockDim.x) {
@@ -505,7 +554,11 @@ route_place_kernel(const RouteParams p) {
   if (blockIdx.x == 0)
     for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = total[e];
   __syncthreads();
-  route_place(p, hist, base);
+  if (at0 >= 0) p.rows[i0] = at0 + base[e0];
+  for (long long i = i0 + blockDim.x; i < c1 * p.k; i += blockDim.x) {
+    const int at = p.rows[i];
+    if (at >= 0) p.rows[i] = at + base[p.ids[i]];
+  }
 }
 
 }  // namespace sk

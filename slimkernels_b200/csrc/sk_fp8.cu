@@ -388,17 +388,16 @@ int launch_route(RouteParams p, int64_t ctas, cudaStream_t stream) {
   // (as many warps as there is work for, four at least: the experts' sums are spread over all threads)
   const int warps = std::min(kRouteWarps, std::max(4, TOPK ? p.per_cta : static_cast<int>(ceil_div(static_cast<int64_t>(p.per_cta) * p.k, 32))));
   const int smem = route_smem_bytes(warps, p.E);
-  const auto allow = [&](auto kern) { return smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess; };
   const auto go = [&](auto per) -> int {
     constexpr int kPer = decltype(per)::value;
     auto kern = ctas == 1 ? route_count_kernel<TYPE, kPer, TOPK, true> : route_count_kernel<TYPE, kPer, TOPK, false>;
-    if (cudaError_t e = allow(kern); e != cudaSuccess) return cuda_status(e);
+    if (smem > 48 * 1024)
+      if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_status(e);
     LaunchConfig lc(ctas, 1, warps * 32, smem, true, 1, stream);
     if (cudaError_t e = cudaLaunchKernelEx(&lc.cfg, kern, p); e != cudaSuccess) return cuda_status(e);
     if (ctas == 1) return SK_OK;
-    if (cudaError_t e = allow(route_place_kernel); e != cudaSuccess) return cuda_status(e);
-    LaunchConfig second(ctas, 1, warps * 32, smem, true, 1, stream);
-    return cuda_status(cudaLaunchKernelEx(&second.cfg, route_place_kernel, p));
+    LaunchConfig second(ctas, 1, 1024, (2 * p.E + 1) * 4, true, 1, stream);
+    return cuda_status(cudaLaunchKernelEx(&second.cfg, route_shift_kernel, p));
   };
   if constexpr (!TOPK) {
     return go(std::integral_constant<int, 1>{});
