@@ -250,6 +250,28 @@ __device__ __forceinline__ void store_row16(uint16_t* dst, int left, int bytes, 
       if (j < left) dst[j] = round_out(value(j), bf16);
   }
 }
+// 128 columns of a warp's 32 rows, one a lane, whose pieces start on 2 bytes only (an odd pitch).  As they lie, 16-bit stores would touch 32 lines
+// each; so the warp turns 16 columns at a time round in its corner of shared memory (kTurnBytes) and a store covers a piece of two rows.
+// dst: the first row; `rows` and `left`: rows and columns that exist.
+constexpr int kTurnPitch = 36, kTurnBytes = 32 * kTurnPitch;
+template <class Value>
+__device__ __forceinline__ void store_rows_turned(uint16_t* dst, long long ld, int rows, int left, uint8_t* corner, int lane, bool bf16, Value&& value) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    if (16 * c >= left) break;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<uint32_t*>(corner + lane * kTurnPitch + 4 * j) = pack_out(value(16 * c + 2 * j), value(16 * c + 2 * j + 1), bf16);
+    __syncwarp();
+    const int col = lane & 15;
+    if (16 * c + col < left) {
+#pragma unroll 4
+      for (int r = lane >> 4; r < rows; r += 2)
+        dst[r * ld + 16 * c + col] = *reinterpret_cast<const uint16_t*>(corner + r * kTurnPitch + 2 * col);
+    }
+  }
+}
 // 32 neighbouring codes of a row (rows start on 32 bytes), values times inv.
 template <class Value>
 __device__ __forceinline__ void store_codes32(uint8_t* dst, int left, float inv, bool bad, Value&& value) {

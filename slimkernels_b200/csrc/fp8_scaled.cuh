@@ -100,15 +100,16 @@ struct Fp8ScaledTraits {
   static constexpr int kNumBars = 2 * kStages + 2 * kSlots + 3;
   static constexpr int kOffMisc = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kOffAmax = kOffMisc + 16;    // SILU: [2 warpgroups][128 rows]
-  static constexpr int kOffTable = kOffAmax + (SILU ? 2 * 128 * 4 : 0);
+  static constexpr int kOffTable = kOffAmax + (SILU ? 2 * 128 * 4 : 8 * kTurnBytes);      // (else the warps' corners)
   static constexpr int kThreads = 512;
   // Registers: 128 a thread at launch; the epilogue holds 128 sums.
   static constexpr int kEpilogueRegs = 184, kOtherRegs = 72;
   static_assert(256 * kEpilogueRegs + 256 * kOtherRegs <= kThreads * 128, "a larger sum would wait forever");
   static constexpr int dynamic_bytes(int experts) { return kOffTable + group_table_bytes(experts) + 1024; }
 };
-static_assert(Fp8ScaledTraits<1, true>::dynamic_bytes(kFp8MaxExperts) <= 232448 && Fp8ScaledTraits<2, true>::dynamic_bytes(kFp8MaxExperts) <= 232448,
+static_assert(Fp8ScaledTraits<1, false>::dynamic_bytes(kFp8MaxExperts) <= 232448 && Fp8ScaledTraits<2, false>::dynamic_bytes(kFp8MaxExperts) <= 232448,
               "shared memory of a CTA");
+static_assert(2 * 128 * 4 <= 8 * kTurnBytes, "(with the SiLU epilogue less)");
 
 template <int CTAS, bool SILU>
 __global__ void __launch_bounds__(512, 1)
@@ -353,6 +354,10 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           for (int c = 0; c < 2; ++c) store_codes32(dst + 32 * c, p.N - n0 - 32 * c, inv, bad, [&](int j) { return h[32 * c + j]; });
           if (wg == 0) store_scale<true>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
         }
+      } else if (p.out_bytes == 2) {
+        const int n0 = t.n * 256 + wg * 128, first = rank * 128 + (warp & 3) * 32;
+        store_rows_turned(static_cast<uint16_t*>(p.out) + (t.row0 + first) * p.ld_out + n0, p.ld_out, min(32, t.rows - first), p.N - n0,
+                          smem + T::kOffAmax + warp * kTurnBytes, lane, p.out_bf16, [&](int j) { return __uint_as_float(v[j >> 5][j & 31]); });
       } else if (live) {
         const int n0 = t.n * 256 + wg * 128;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + m * p.ld_out + n0;

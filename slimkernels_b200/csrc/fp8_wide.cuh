@@ -37,14 +37,15 @@ struct Fp8WideTraits {
   static constexpr int kOffXScale = kOffMisc + 16;  // [kSlots][256 epilogue threads][4]
   static constexpr int kOffWScale = kOffXScale + kSlots * 256 * 16;      // [kSlots][8 warps][2 weight blocks][4]
   static constexpr int kOffAmax = kOffWScale + kSlots * 8 * 32;          // SILU: [2 warpgroups][128 rows]
-  static constexpr int kOffTable = kOffAmax + (SILU ? 2 * 128 * 4 : 0);
+  static constexpr int kOffTable = kOffAmax + (SILU ? 2 * 128 * 4 : 8 * kTurnBytes);      // (else the warps' corners)
   static constexpr int kThreads = 384;             // two epilogue warpgroups, one for the producer and the issuer
   // Registers: 168 a thread at launch; the epilogue's 128 sums and 32 loaded values take more, the other roles less.
   static constexpr int kEpilogueRegs = 232, kOtherRegs = 40;
   static_assert(256 * kEpilogueRegs + 128 * kOtherRegs <= kThreads * 168, "a larger sum would wait forever");
   static constexpr int dynamic_bytes(int experts) { return kOffTable + group_table_bytes(experts) + 1024; }
 };
-static_assert(Fp8WideTraits<true>::dynamic_bytes(kFp8MaxExperts) <= 232448, "shared memory of a CTA");
+static_assert(Fp8WideTraits<true>::dynamic_bytes(kFp8MaxExperts) <= 232448 && Fp8WideTraits<false>::dynamic_bytes(kFp8MaxExperts) <= 232448,
+              "shared memory of a CTA");
 
 template <bool SILU>
 __global__ void __launch_bounds__(384, 1)
@@ -265,6 +266,10 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           for (int c = 0; c < 2; ++c) store_codes32(dst + 32 * c, p.N - n0 - 32 * c, inv, bad, [&](int j) { return acc[32 * c + j]; });
           if (wg == 0) store_scale<false>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
         }
+      } else if (p.out_bytes == 2) {
+        const int n0 = t.n * 256 + wg * 128, first = (warp & 3) * 32;
+        store_rows_turned(static_cast<uint16_t*>(p.out) + (t.row0 + first) * p.ld_out + n0, p.ld_out, min(32, t.rows - first), p.N - n0,
+                          smem + T::kOffAmax + warp * kTurnBytes, lane, p.out_bf16, [&](int j) { return acc[j]; });
       } else if (live) {
         const int n0 = t.n * 256 + wg * 128;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + m * p.ld_out + n0;
