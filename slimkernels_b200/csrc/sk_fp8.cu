@@ -170,7 +170,9 @@ struct Choice {
 //     tile 16  21.9 / 27.0 / 33.4 / 47.8     many  28.7 / 29.8 / 31.0 / 31.4
 //   With the SiLU epilogue, whose time goes with the tile's rows, tiles of 16 are the fastest up to 32 rows per expert (67 us a block, tiles of 32 87, many 80).
 // A tile's K range is split while that leaves an SM for every CTA and a CTA eight K blocks or so: 64 x 4096 x 4096 12.9 us in one, 10.9 in four; splitting
-// where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two).
+// where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two; 256 x 2048 x 4096, 8-bit scales, 11.1 and 11.7).  Two CTAs to an SM
+// are better only where K is long -- 32-bit scales: 100 x 1000 x 8192 13.2 in two, 9.6 in four; 300 x 512 x 16384 33.5 in one, 22.4 in two; 8-bit scales: 300 x 512
+// x 16384 19.6 in two, 14.1 in four; 16 x 8192 x 16384 26.7 and 24.8; but 100 x 1000 x 8192 9.1 in four and in eight.
 Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, int sms) {
   Choice c;
   const int64_t rows = ceil_div(M, experts);       // of a group, on average
@@ -199,6 +201,7 @@ Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bo
   c.split = 1;
   if (!grouped && few) {
     while (c.split < 8 && tiles * c.split * 2 <= sms && kb >= c.split * 8) c.split *= 2;
+    while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * (e8m0 ? 64 : 32)) c.split *= 2;
     if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
   }
   c.ctas = tiles * c.split;

@@ -220,6 +220,8 @@ def test_launches_are_what_the_rules_say(forced):
     assert query(64 * 20, 2048, 2048, 64, F32)[0] == capi.FP8_MANY
     kernel, tile, features, split, ctas = query(5, 1024, 8192)
     assert ctas == 8 * split and ctas <= sms and split == 8
+    assert query(300, 512, 16384)[:4] == [capi.FP8_FEW, 32, 128, 4] and query(300, 512, 16384, scales=F32)[:4] == [capi.FP8_FEW, 16, 128, 2]
+    assert query(256, 2048, 4096)[3] == 1 and query(16, 22016, 4096)[3] == 1 and query(100, 1000, 8192, scales=F32)[3] == 4
     for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 1, 2000)):
         assert lib.sk_fp8_query_launch(*bad, 0, None, None, None, None, None) == capi.SK_ERR_BAD_SHAPE
     forced(kernel=capi.FP8_PAIR)
@@ -439,6 +441,34 @@ def test_linear_layers_past_32_bits(M, N, K, scales):
     for part in (slice(0, 20), slice(M - 70, M)):
         exact, tol = F.product_tolerance(F.quantised_values(x[part]), F.weight_values(*w), torch.bfloat16)
         F.assert_within(y[part], exact, tol)
+
+
+@pytest.mark.parametrize("M,N,K,scales", [(594, 256, 10608, F32), (300, 512, 16384, E8M0), (100, 1000, 8192, F32), (16, 8192, 16384, E8M0)])
+def test_split_products_of_two_ctas_to_an_sm(M, N, K, scales):
+    x = _operands(M, N, K, scales, 5)
+    y = sk.fp8_gemm(*x)
+    exact, tol = F.product_tolerance(F.row_values(*x[:2]), F.weight_values(*x[2:]), torch.bfloat16)
+    F.assert_within(y, exact, tol)
+    assert torch.equal(y, sk.fp8_gemm(*x))
+
+
+@pytest.mark.parametrize("kernel", [capi.FP8_MANY, capi.FP8_PAIR])
+@pytest.mark.parametrize("scales", [E8M0, F32])
+def test_odd_pitches_write_their_rows_and_columns_only(kernel, scales, forced):
+    """Results whose rows start on 2 bytes, by groups that end inside a warp's rows, into a slice of a larger matrix."""
+    g = F.generator(16)
+    off = torch.tensor([0, 1, 34, 34, 200, 331], dtype=torch.int32, device="cuda")
+    w = sk.prepare_weight_fp8(torch.randn(5, 413, 256, generator=g, device="cuda"), scales)
+    x = sk.quantize_fp8(torch.randn(340, 256, generator=g, device="cuda"), scales)
+    forced(kernel=kernel)
+    want = torch.zeros(340, 416, dtype=torch.bfloat16, device="cuda")[:, :413]
+    sk.fp8_grouped_gemm(*x, *w, off, out=want)
+    whole = torch.full((345, 421), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = whole[3:343, 5:418]
+    sk.fp8_grouped_gemm(*x, *w, off, out=out)
+    assert torch.equal(out[:331], want[:331])
+    out[:331] = 7.0
+    assert bool((whole == 7.0).all())
 
 
 @pytest.mark.parametrize("kernel", [capi.FP8_FEW, capi.FP8_MANY, capi.FP8_PAIR])
