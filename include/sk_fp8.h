@@ -82,7 +82,7 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
  *   y_e(x) = W_down[e] q( SiLU(gate) * up ),   [gate; up] = W_gate_up[e] q(x),   q the quantiser above,
  *   out[t] = cast( sum_j weights[t, j] * y_{expert of (t, j)}(x[t]) ),   choices with rows outside [0, T * k) count nothing.
  * gate_up: 2 * experts matrices [inter, hidden] (an expert's gate, then its up; `experts` there counts matrices), down: experts
- * matrices [hidden, inter].  y is rounded to out_dtype before it is summed.  x_type: fp16 or bf16 or fp32.  rows and offsets are those of
+ * matrices [hidden, inter].  y and its sum are fp32, rounded once.  x_type: fp16 or bf16 or fp32.  rows and offsets are those of
  * one routing: a place that lies in no group has no result.  The workspace is 256-byte aligned. */
 int64_t sk_fp8_experts_workspace_bytes(int64_t T, int64_t k, int64_t hidden, int64_t inter, int scale_type);
 int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x, const int32_t* rows, const float* weights,

@@ -24,7 +24,7 @@ struct Fp8Params {
   const int* offsets;                   // [experts + 1] first rows of the groups, or nullptr: one group of all rows
   int experts;
   int w_rows;                           // weight rows per expert
-  void* out;                            // [M, ld_out] half / bf16; with the SiLU epilogue: e4m3 codes
+  void* out;                            // [M, ld_out] half / bf16 / fp32; with the SiLU epilogue: e4m3 codes
   long long ld_out;
   void* h_scale;                        // SiLU epilogue: the codes' scales, element (m, b) at m * hs_row + b * hs_blk
   long long hs_row, hs_blk;
@@ -34,6 +34,7 @@ struct Fp8Params {
   int up_row0;                          // SiLU epilogue: the up projection's first row / scale block within an expert
   int up_block0;
   int out_bf16;
+  int out_f32;                          // the result is kept in fp32 (the expert layers' second product; rows on 64 bytes)
   int x_scale_groups, w_scale_groups;   // the scales of four K blocks may be loaded at once (side by side and aligned)
   int out_bytes;                        // what the rows of the result start on: 32, 16 or 2 bytes
   int early_weights;                    // the weights may be read before the previous kernel is complete
@@ -248,6 +249,23 @@ __device__ __forceinline__ void store_row16(uint16_t* dst, int left, int bytes, 
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       if (j < left) dst[j] = round_out(value(j), bf16);
+  }
+}
+// The same in fp32; rows and pieces start on 64 bytes.
+template <class Value>
+__device__ __forceinline__ void store_row16_f32(float* dst, int left, Value&& value) {
+  if (left >= 16) {
+#pragma unroll
+    for (int h = 0; h < 16; h += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(value(h + j));
+      st_global_v8(dst + h, w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < left) dst[j] = value(j);
   }
 }
 // 128 columns of a warp's 32 rows, one a lane, whose pieces start on 2 bytes only (an odd pitch).  As they lie, 16-bit stores would touch 32 lines

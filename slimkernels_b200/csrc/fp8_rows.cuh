@@ -172,9 +172,11 @@ fp8_prepare_weight_kernel(const void* w, long long ld_w, long long matrix, int N
 }
 
 // out[t, :] = round( sum over j of weights[t, j] * y[rows[t, j], :] ), in the order of j; choices with rows outside [0, T * choices) count nothing.
+// y is fp32, as the second product leaves it: the result is rounded once, and an expert's result past fp16's range is no infinity in a sum
+// within it.
 template <bool BF16, bool VECTOR>
 __global__ void __launch_bounds__(256)
-fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const float* weights, int choices, int T, int H, uint16_t* out,
+fp8_combine_kernel(const float* y, long long ld_y, const int* rows, const float* weights, int choices, int T, int H, uint16_t* out,
                    long long ld_out) {
   grid_dep_wait();
   grid_dep_launch_dependents();
@@ -191,11 +193,11 @@ fp8_combine_kernel(const uint16_t* y, long long ld_y, const int* rows, const flo
       const float w = ld_global_f32(weights + t * choices + j);
       if constexpr (VECTOR) {
         float f[8];
-        load_eight<BF16 ? 1 : 0>(y, r * ld_y + h, f);
+        load_eight<2>(y, r * ld_y + h, f);
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, f[c], acc[c]);
       } else {
-        acc[0] = fmaf(w, load_element<BF16 ? 1 : 0>(y, r * ld_y + h), acc[0]);
+        acc[0] = fmaf(w, load_element<2>(y, r * ld_y + h), acc[0]);
       }
     }
     uint16_t* dst = out + t * ld_out + h;

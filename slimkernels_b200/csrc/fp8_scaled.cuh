@@ -354,6 +354,14 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           for (int c = 0; c < 2; ++c) store_codes32(dst + 32 * c, p.N - n0 - 32 * c, inv, bad, [&](int j) { return h[32 * c + j]; });
           if (wg == 0) store_scale<true>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
         }
+      } else if (p.out_f32) {
+        const int n0 = t.n * 256 + wg * 128;
+        float* dst = static_cast<float*>(p.out) + m * p.ld_out + n0;
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            store_row16_f32(dst + 16 * c, p.N - n0 - 16 * c, [&](int j) { return __uint_as_float(v[c >> 1][16 * (c & 1) + j]); });
+        }
       } else if (p.out_bytes == 2) {
         const int n0 = t.n * 256 + wg * 128, first = rank * 128 + (warp & 3) * 32;
         store_rows_turned(static_cast<uint16_t*>(p.out) + (t.row0 + first) * p.ld_out + n0, p.ld_out, min(32, t.rows - first), p.N - n0,

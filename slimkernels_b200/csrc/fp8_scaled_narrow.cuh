@@ -303,6 +303,11 @@ fp8_scaled_narrow_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
 #pragma unroll
         for (int j = 0; j < TOK; ++j)
           st_dsmem_f32(map_to_cta(red_at + static_cast<uint32_t>(j & ((1 << shift) - 1)) * 512, j >> shift), sum(0, j));
+      } else if (n < p.N && p.out_f32) {
+        float* out = static_cast<float*>(p.out) + static_cast<long long>(t.row0) * p.ld_out + n;
+#pragma unroll
+        for (int j = 0; j < TOK; ++j)
+          if (j < t.rows) out[j * p.ld_out] = sum(0, j);
       } else if (n < p.N) {
         uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<long long>(t.row0) * p.ld_out + n;
 #pragma unroll

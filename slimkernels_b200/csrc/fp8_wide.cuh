@@ -266,6 +266,13 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           for (int c = 0; c < 2; ++c) store_codes32(dst + 32 * c, p.N - n0 - 32 * c, inv, bad, [&](int j) { return acc[32 * c + j]; });
           if (wg == 0) store_scale<false>(p.h_scale, m * p.hs_row + t.n * p.hs_blk, e, bad);
         }
+      } else if (p.out_f32) {
+        const int n0 = t.n * 256 + wg * 128;
+        float* dst = static_cast<float*>(p.out) + m * p.ld_out + n0;
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) store_row16_f32(dst + 16 * c, p.N - n0 - 16 * c, [&](int j) { return acc[16 * c + j]; });
+        }
       } else if (p.out_bytes == 2) {
         const int n0 = t.n * 256 + wg * 128, first = (warp & 3) * 32;
         store_rows_turned(static_cast<uint16_t*>(p.out) + (t.row0 + first) * p.ld_out + n0, p.ld_out, min(32, t.rows - first), p.N - n0,

@@ -92,6 +92,7 @@ int codes_map(const void* q, int64_t rows, int64_t K, int64_t ld, int box_rows, 
 constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 constexpr int64_t kIntMax = 0x7fffffff;
+constexpr int kOutF32 = -1;             // beside sk_out_dtype: the expert layers' second product, whose results a weighted sum follows
 bool aligned(const void* p, int64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool is_scale_type(int t) { return t == SK_SCALE_F32 || t == SK_SCALE_E8M0; }
 bool is_float_type(int t) { return t >= SK_FLOAT_F16 && t <= SK_FLOAT_F32; }
@@ -308,6 +309,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   p.k_blocks = static_cast<int>(ceil_div(K, 128));
   p.n_tiles = static_cast<int>(ceil_div(N, c.feature_tile));
   p.out_bf16 = out_dtype == SK_OUT_BF16;
+  p.out_f32 = out_dtype == kOutF32;
   p.out_bytes = silu ? 32 : aligned(out, 32) && ld_out % 16 == 0 ? 32 : aligned(out, 16) && ld_out % 8 == 0 ? 16 : 2;
   const int64_t four = 4 * scale_bytes(scale_type);
   p.x_scale_groups = p.xs_blk == 1 && p.xs_row % 4 == 0 && aligned(p.x_scale, four);
@@ -559,7 +561,7 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
 
 int64_t sk_fp8_experts_workspace_bytes(int64_t T, int64_t k, int64_t hidden, int64_t inter, int scale_type) {
   if (T < 0 || k < 1 || hidden < 1 || inter < 1 || !is_scale_type(scale_type)) return 0;
-  return rows_bytes(T * k, hidden, scale_type) + rows_bytes(T * k, inter, scale_type) + round_up(T * k * round_up(hidden, 16) * 2, 256);
+  return rows_bytes(T * k, hidden, scale_type) + rows_bytes(T * k, inter, scale_type) + round_up(T * k * round_up(hidden, 16) * 4, 256);
 }
 
 int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x, const int32_t* rows, const float* weights, const int32_t* offsets,
@@ -584,7 +586,7 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
   at += rows_bytes(R, inter, scale_type);
   if (int rc = quantize(x, x_type, ld_x, T, hidden, xr, scale_type, rows, k, s); rc != SK_OK) return rc;
   if (int rc = product(R, &xr, gate_up, scale_type, offsets, nullptr, 0, out_dtype, &hr, true, s); rc != SK_OK) return rc;
-  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, out_dtype, nullptr, true, s); rc != SK_OK) return rc;
+  if (int rc = product(R, &hr, down, scale_type, offsets, at, ld_y, kOutF32, nullptr, true, s); rc != SK_OK) return rc;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
   const bool vector = hidden % 8 == 0 && ld_out % 8 == 0 && aligned(out, 16);
@@ -593,7 +595,7 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
   return with_bool(out_dtype == SK_OUT_BF16, [&](auto bf16) {
     return with_bool(vector, [&](auto v) {
       return cuda_status(cudaLaunchKernelEx(&lc.cfg, fp8_combine_kernel<decltype(bf16)::value, decltype(v)::value>,
-                                            reinterpret_cast<const uint16_t*>(at), static_cast<long long>(ld_y), static_cast<const int*>(rows), weights,
+                                            reinterpret_cast<const float*>(at), static_cast<long long>(ld_y), static_cast<const int*>(rows), weights,
                                             static_cast<int>(k), static_cast<int>(T), static_cast<int>(hidden), static_cast<uint16_t*>(out),
                                             static_cast<long long>(ld_out)));
     });

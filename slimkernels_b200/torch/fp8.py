@@ -97,7 +97,7 @@ def fp8_experts(x, routing: Routing, gate_up, gate_up_scale, down, down_scale, o
 
     x [..., hidden] with T tokens in all, gate_up codes [E, 2, inter, hidden] (gate first), down codes [E, hidden, inter].  Four
     kernels: quantise into the groups' rows, grouped product with SiLU * up and the re-quantisation in its epilogue, grouped
-    product, weighted sum.
+    product, weighted sum.  The experts' results and their sum are fp32, rounded once.
     """
     return _op("fp8_experts")(x, routing.rows, routing.weights, routing.offsets, gate_up, gate_up_scale, down, down_scale, out_dtype)
 
