@@ -477,8 +477,9 @@ __device__ __forceinline__ int warp_scan(int n, int lane) {
   }
   return n;
 }
+constexpr int kRouteStaticBytes = 32 * 4;
 __device__ __forceinline__ void scan_experts(int* total, int E) {
-  __shared__ int ahead[32];
+  __shared__ int ahead[kRouteStaticBytes / 4];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = (E + 31) >> 5;
   for (int g = warp; g < parts; g += warps) {
     const int e = 32 * g + lane, n = e < E ? total[e] : 0, incl = warp_scan(n, lane);

@@ -396,7 +396,7 @@ int launch_route(RouteParams p, int64_t ctas, cudaStream_t stream) {
   const auto go = [&](auto per) -> int {
     constexpr int kPer = decltype(per)::value;
     auto kern = ctas == 1 ? route_count_kernel<TYPE, kPer, TOPK, true> : route_count_kernel<TYPE, kPer, TOPK, false>;
-    if (smem > 48 * 1024)
+    if (smem + kRouteStaticBytes > 48 * 1024)         // (what a launch may have without asking counts both)
       if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_status(e);
     LaunchConfig lc(ctas, 1, warps * 32, smem, true, 1, stream);
     if (cudaError_t e = cudaLaunchKernelEx(&lc.cfg, kern, p); e != cudaSuccess) return cuda_status(e);

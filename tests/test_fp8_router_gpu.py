@@ -1,16 +1,11 @@
-"""Launches of the router: tables that fill the shared memory a kernel has without asking, and calls from several host threads."""
+"""Launches of the router whose tables fill the shared memory that a kernel has without asking for more."""
 import subprocess
 import sys
-import threading
 
-import numpy as np
 import pytest
 import torch
 
-import fp8_util as F
-import slimkernels_b200.torch as sk
 from conftest import ROOT
-from slimkernels_b200 import capi
 
 pytestmark = pytest.mark.gpu
 
