@@ -477,9 +477,8 @@ __device__ __forceinline__ int warp_scan(int n, int lane) {
   }
   return n;
 }
-constexpr int kRouteStaticBytes = 32 * 4;
 __device__ __forceinline__ void scan_experts(int* total, int E) {
-  __shared__ int ahead[kRouteStaticBytes / 4];
+  __shared__ int ahead[32];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = (E + 31) >> 5;
   for (int g = warp; g < parts; g += warps) {
     const int e = 32 * g + lane, n = e < E ? total[e] : 0, incl = warp_scan(n, lane);
@@ -498,6 +497,7 @@ __device__ __forceinline__ void scan_experts(int* total, int E) {
 
 // Shared memory of pass 1: [warps][E] counts, [E + 1] first places.
 __host__ __device__ constexpr int route_smem_bytes(int warps, int E) { return (warps * E + E + 1) * 4; }
+static_assert(route_smem_bytes(kRouteWarps, kFp8MaxExperts) + 128 <= 232448, "shared memory of a CTA (128 bytes are scan_experts')");
 
 template <int TYPE, int PER, bool TOPK, bool ONE_CTA>
 __global__ void __launch_bounds__(kRouteWarps * 32)

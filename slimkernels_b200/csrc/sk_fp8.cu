@@ -389,15 +389,16 @@ int64_t route_per_cta(int64_t T, int sms) {
 }
 
 template <int TYPE, bool TOPK>
-int launch_route(RouteParams p, int64_t ctas, cudaStream_t stream) {
+int launch_route(RouteParams p, int64_t ctas, const DeviceInfo& dev, cudaStream_t stream) {
   // (as many warps as there is work for, four at least: the experts' sums are spread over all threads)
   const int warps = std::min(kRouteWarps, std::max(4, TOPK ? p.per_cta : static_cast<int>(ceil_div(static_cast<int64_t>(p.per_cta) * p.k, 32))));
   const int smem = route_smem_bytes(warps, p.E);
   const auto go = [&](auto per) -> int {
     constexpr int kPer = decltype(per)::value;
     auto kern = ctas == 1 ? route_count_kernel<TYPE, kPer, TOPK, true> : route_count_kernel<TYPE, kPer, TOPK, false>;
-    if (smem + kRouteStaticBytes > 48 * 1024)         // (what a launch may have without asking counts both)
-      if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_status(e);
+    // (what any call may want, not what this one does: the limit is the kernel's, and another thread may be about to launch it)
+    static std::atomic<uint64_t> done[2];
+    if (int rc = allow_shared(kern, route_smem_bytes(kRouteWarps, kFp8MaxExperts), dev, done[ctas == 1]); rc != SK_OK) return rc;
     LaunchConfig lc(ctas, 1, warps * 32, smem, true, 1, stream);
     if (cudaError_t e = cudaLaunchKernelEx(&lc.cfg, kern, p); e != cudaSuccess) return cuda_status(e);
     if (ctas == 1) return SK_OK;
@@ -431,8 +432,8 @@ int route(RouteParams p, int logits_type, bool topk, int64_t T, int64_t E, int64
     if (!aligned(workspace, 4)) return SK_ERR_BAD_ALIGNMENT;
     p.counts = static_cast<int*>(workspace);
   }
-  if (!topk) return launch_route<0, false>(p, ctas, stream);
-  return with_type(logits_type, [&](auto type) { return launch_route<decltype(type)::value, true>(p, ctas, stream); });
+  if (!topk) return launch_route<0, false>(p, ctas, dev, stream);
+  return with_type(logits_type, [&](auto type) { return launch_route<decltype(type)::value, true>(p, ctas, dev, stream); });
 }
 
 int check_route(int64_t T, int64_t E, int64_t k) {
