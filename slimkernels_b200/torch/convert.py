@@ -30,11 +30,13 @@ def _convertible(linear: nn.Linear, group_size: int) -> bool:
     return linear.in_features % group_size == 0 and linear.in_features % 32 == 0
 
 
+_MLP_NAMES = ("gate_proj", "up_proj", "down_proj")
+
+
 def _is_llama_mlp(module: nn.Module) -> bool:
-    names = ("gate_proj", "up_proj", "down_proj")
-    if not all(isinstance(getattr(module, n, None), nn.Linear) for n in names):
+    if not all(isinstance(getattr(module, n, None), nn.Linear) for n in _MLP_NAMES):
         return False
-    if any(getattr(module, n).bias is not None for n in names):
+    if any(getattr(module, n).bias is not None for n in _MLP_NAMES):
         return False
     return _is_silu(getattr(module, "act_fn", None))
 
@@ -63,7 +65,8 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
                      device=None, fp8=(), experts: bool = False) -> dict:
     """Replace, in place, every `nn.Linear` whose in_features is a multiple of `group_size` (except names in `skip`).
 
-    fp8: names of `nn.Linear` layers that become `FP8Linear` instead, whatever `skip` says (fp8=("lm_head",) for the output head).
+    fp8: names of `nn.Linear` layers that become `FP8Linear` instead, whatever `skip` says (fp8=("lm_head",) for the output head).  An MLP
+    block with a layer among them is not fused.
     experts: stacked expert weights (see _is_experts) become `FP8Experts`.
 
     Returns {"linear": n, "mlp": n, "kept": [names left as they were]}, with `fp8` or `experts` also their numbers.  The model must be on
@@ -75,6 +78,9 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
     if experts:
         stats["experts"] = 0
 
+    def in_fp8(name, full):
+        return name in fp8 or full in fp8
+
     def dev_of(linear):
         return device if device is not None else linear.weight.device
 
@@ -85,7 +91,7 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
     def walk(parent: nn.Module, prefix: str):
         for name, child in list(parent.named_children()):
             full = f"{prefix}{name}"
-            if isinstance(child, nn.Linear) and (name in fp8 or full in fp8):
+            if isinstance(child, nn.Linear) and in_fp8(name, full):
                 setattr(parent, name, FP8Linear.from_float(child.weight, child.bias, dev_of(child), _out_dtype(child.weight)))
                 stats["fp8"] += 1
                 continue
@@ -93,7 +99,7 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
                 stats["kept"].append(full)
                 continue
             if fuse_mlp and _is_llama_mlp(child) and _convertible(child.gate_proj, group_size) \
-                    and _convertible(child.down_proj, group_size):
+                    and _convertible(child.down_proj, group_size) and not any(in_fp8(n, f"{full}.{n}") for n in _MLP_NAMES):
                 gate_up = torch.cat([child.gate_proj.weight, child.up_proj.weight], dim=0)   # gate rows first
                 fused = W2A8LlamaMLP(W2A8Linear.from_float(gate_up, group_size, device=dev_of(child.gate_proj)),
                                      W2A8Linear.from_float(child.down_proj.weight, group_size,
