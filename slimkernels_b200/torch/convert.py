@@ -66,7 +66,7 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
     """Replace, in place, every `nn.Linear` whose in_features is a multiple of `group_size` (except names in `skip`).
 
     fp8: names of `nn.Linear` layers that become `FP8Linear` instead, whatever `skip` says (fp8=("lm_head",) for the output head).  An MLP
-    block with a layer among them is not fused.
+    block with a layer among them is not fused, and of a module that `skip` names they alone are converted (it counts as kept).
     experts: stacked expert weights (see _is_experts) become `FP8Experts`.
 
     Returns {"linear": n, "mlp": n, "kept": [names left as they were]}, with `fp8` or `experts` also their numbers.  The model must be on
@@ -88,15 +88,17 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
         q = W2A8Linear.from_float(linear.weight, group_size, device=dev_of(linear))
         return q if linear.bias is None else _W2A8LinearWithBias(q, linear.bias.to(dev_of(linear)))
 
-    def walk(parent: nn.Module, prefix: str):
+    def walk(parent: nn.Module, prefix: str, skipped: bool = False):
         for name, child in list(parent.named_children()):
             full = f"{prefix}{name}"
             if isinstance(child, nn.Linear) and in_fp8(name, full):
                 setattr(parent, name, FP8Linear.from_float(child.weight, child.bias, dev_of(child), _out_dtype(child.weight)))
                 stats["fp8"] += 1
                 continue
-            if name in skip or full in skip:
-                stats["kept"].append(full)
+            if skipped or name in skip or full in skip:
+                if not skipped:
+                    stats["kept"].append(full)
+                walk(child, full + ".", True)
                 continue
             if fuse_mlp and _is_llama_mlp(child) and _convertible(child.gate_proj, group_size) \
                     and _convertible(child.down_proj, group_size) and not any(in_fp8(n, f"{full}.{n}") for n in _MLP_NAMES):

@@ -66,3 +66,17 @@ def test_a_full_name_opens_one_block_only():
     assert stats == {"linear": 4, "mlp": 1, "kept": ["lm_head"], "fp8": 1}
     kinds = _kinds(m)
     assert kinds["layers.0.mlp"] == "mlp" and kinds["layers.1.mlp.down_proj"] == "8-bit" and kinds["layers.1.mlp.up_proj"] == "2-bit"
+
+
+def test_names_below_a_skipped_module_are_converted():
+    m = _Model()
+    stats = convert.quantize_linears(m, skip=("mlp", "lm_head"), fp8=("down_proj",))
+    assert stats == {"linear": 2, "mlp": 0, "kept": ["layers.0.mlp", "layers.1.mlp", "lm_head"], "fp8": 2}
+    assert _kinds(m) == {f"layers.{i}.{n}": kind for i in (0, 1) for n, kind in (("q_proj", "2-bit"), ("mlp.down_proj", "8-bit"))}
+
+
+def test_a_skipped_module_is_left_alone_otherwise():
+    m = _Model()
+    m.layers[0].mlp.gate_up_proj, m.layers[0].mlp.down = nn.Parameter(torch.zeros(2, 8, 4)), nn.Linear(128, 128)
+    convert.quantize_linears(m, skip=("layers",), fp8=("layers.1.q_proj",), experts=True)
+    assert _kinds(m) == {"layers.1.q_proj": "8-bit"}
