@@ -78,5 +78,5 @@ def test_names_below_a_skipped_module_are_converted():
 def test_a_skipped_module_is_left_alone_otherwise():
     m = _Model()
     m.layers[0].mlp.gate_up_proj, m.layers[0].mlp.down = nn.Parameter(torch.zeros(2, 8, 4)), nn.Linear(128, 128)
-    convert.quantize_linears(m, skip=("layers",), fp8=("layers.1.q_proj",), experts=True)
+    convert.quantize_linears(m, skip=("layers", "lm_head"), fp8=("layers.1.q_proj",), experts=True)
     assert _kinds(m) == {"layers.1.q_proj": "8-bit"}
