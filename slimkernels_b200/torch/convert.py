@@ -66,12 +66,18 @@ def quantize_linears(model: nn.Module, group_size: int = 128, skip=("lm_head",),
     """Replace, in place, every `nn.Linear` whose in_features is a multiple of `group_size` (except names in `skip`).
 
     fp8: names of `nn.Linear` layers that become `FP8Linear` instead, whatever `skip` says (fp8=("lm_head",) for the output head).  An MLP
-    block with a layer among them is not fused, and of a module that `skip` names they alone are converted (it counts as kept).
+    block with a layer among them is not fused, and of a module that `skip` names they alone are converted (it counts as kept).  A name that
+    fits no layer is an error.
     experts: stacked expert weights (see _is_experts) become `FP8Experts`.
 
     Returns {"linear": n, "mlp": n, "kept": [names left as they were]}, with `fp8` or `experts` also their numbers.  The model must be on
     a CUDA device (or `device` given): quantisation runs there.
     """
+    fp8 = (fp8,) if isinstance(fp8, str) else tuple(fp8)
+    linears = [full for full, m in model.named_modules(remove_duplicate=False) if isinstance(m, (nn.Linear, FP8Linear))]
+    unknown = [n for n in fp8 if not any(n in (full, full.rpartition(".")[2]) for full in linears)]
+    if unknown:
+        raise ValueError(f"fp8 names layers that are no nn.Linear of this model: {unknown}")
     stats = {"linear": 0, "mlp": 0, "kept": []}
     if fp8:
         stats["fp8"] = 0

@@ -80,3 +80,24 @@ def test_a_skipped_module_is_left_alone_otherwise():
     m.layers[0].mlp.gate_up_proj, m.layers[0].mlp.down = nn.Parameter(torch.zeros(2, 8, 4)), nn.Linear(128, 128)
     convert.quantize_linears(m, skip=("layers", "lm_head"), fp8=("layers.1.q_proj",), experts=True)
     assert _kinds(m) == {"layers.1.q_proj": "8-bit"}
+
+
+@pytest.mark.parametrize("names", [("lm_haed",), ("lm_head", "layers.2.q_proj"), ("mlp",), ("embed",)])
+def test_names_of_no_linear_layer_are_refused_before_anything_is_converted(names):
+    m = _Model()
+    with pytest.raises(ValueError, match=names[-1]):
+        convert.quantize_linears(m, fp8=names)
+    assert _kinds(m) == {}
+
+
+def test_one_name_may_stand_alone():
+    m = _Model()
+    m.head = nn.Linear(100, 8)                              # (its name is a part of the other's)
+    stats = convert.quantize_linears(m, fp8="lm_head")
+    assert stats["fp8"] == 1 and _kinds(m)["lm_head"] == "8-bit" and stats["kept"] == ["head"]
+
+
+def test_a_layer_that_is_converted_already_keeps_its_name():
+    m = _Model()
+    m.lm_head = convert.FP8Linear(torch.zeros(32, 128, dtype=torch.float8_e4m3fn), torch.ones(1, 1), 128)
+    assert convert.quantize_linears(m, fp8=("lm_head",))["fp8"] == 0 and isinstance(m.lm_head, convert.FP8Linear)
