@@ -89,7 +89,7 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
                    const int32_t* offsets, const sk_fp8_weight* gate_up, const sk_fp8_weight* down, int scale_type, void* out,
                    int64_t ld_out, int out_dtype, void* workspace, int64_t workspace_bytes, sk_stream_t stream);
 
-/* Reads and clears (synchronously) the word in which a kernel of this header notes a wait that ran into its limit on `device`;
+/* Waits for all work on `device`, then reads and clears the word in which a kernel of this header notes a wait that ran into its limit there;
  * non-zero maps to SK_ERR_DEVICE_TIMEOUT.  sk_device_status_string words it.  The output of such a launch is undefined. */
 int sk_fp8_last_device_status(int device, int* device_status);
 typedef enum sk_fp8_kernel {

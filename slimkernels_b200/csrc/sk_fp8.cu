@@ -610,7 +610,10 @@ int sk_fp8_last_device_status(int device, int* device_status) {
   if (cudaError_t e = cudaSetDevice(device); e != cudaSuccess) return cuda_status(e);
   int word = 0;
   const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&word, g_fp8_status, sizeof(int));
+  // (the copy alone would wait for streams that synchronise with the legacy one, and others may still run into their limit)
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&word, g_fp8_status, sizeof(int));
+  // (while the word is not zero, kernels leave it as it is: nothing noted in between is lost)
   if (e == cudaSuccess && word != 0) e = cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int));
   (void)cudaSetDevice(cur);
   if (e != cudaSuccess) return cuda_status(e);

@@ -103,7 +103,8 @@ def fp8_experts(x, routing: Routing, gate_up, gate_up_scale, down, down_scale, o
 
 
 def fp8_device_status(device=None) -> int:
-    """Reads and clears the device's note of a wait inside an FP8 kernel that ran into its limit (0: none).  Synchronises."""
+    """Reads and clears the device's note of a wait inside an FP8 kernel that ran into its limit (0: none).  Waits for all
+    streams of the device."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     return _op("fp8_device_status")(torch.cuda.current_device() if index is None else index)
 
