@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 #include "../../include/sk_fp8.h"
 #include "fp8_common.cuh"
@@ -94,6 +95,9 @@ constexpr int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 constexpr int64_t kIntMax = 0x7fffffff;
 constexpr int kOutF32 = -1;             // beside sk_out_dtype: the expert layers' second product, whose results a weighted sum follows
 bool aligned(const void* p, int64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool aligned4(std::initializer_list<const void*> ps) {
+  return std::all_of(ps.begin(), ps.end(), [](const void* p) { return aligned(p, 4); });
+}
 bool is_scale_type(int t) { return t == SK_SCALE_F32 || t == SK_SCALE_E8M0; }
 bool is_float_type(int t) { return t >= SK_FLOAT_F16 && t <= SK_FLOAT_F32; }
 bool is_out_type(int t) { return t == SK_OUT_F16 || t == SK_OUT_BF16; }
@@ -453,7 +457,7 @@ int sk_fp8_quantize(const void* x, int x_type, int64_t ld_x, int64_t M, int64_t 
   if (!is_float_type(x_type) || !is_scale_type(scale_type)) return SK_ERR_BAD_ARGUMENT;
   if (K < 1 || K > kIntMax / 256 || ld_x < K) return SK_ERR_BAD_SHAPE;
   if (int rc = check_rows(out, M, K); rc != SK_OK) return rc;
-  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2)) return SK_ERR_BAD_ALIGNMENT;
+  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2) || (scale_type == SK_SCALE_F32 && !aligned(out->scale, 4))) return SK_ERR_BAD_ALIGNMENT;
   if (M == 0) return SK_OK;
   return quantize(x, x_type, ld_x, M, K, *out, scale_type, nullptr, 1, static_cast<cudaStream_t>(stream));
 }
@@ -466,6 +470,7 @@ int sk_fp8_prepare_weight(const void* w, int w_type, int64_t ld_w, int64_t w_mat
   const int64_t blocks = ceil_div(N, 128) * ceil_div(K, 128);
   if (blocks > kIntMax) return SK_ERR_BAD_SHAPE;
   if (!aligned(w, w_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(w_q, 16) || ld_q % 16 || q_matrix % 4) return SK_ERR_BAD_ALIGNMENT;
+  if (scale_type == SK_SCALE_F32 && !aligned(w_scale, 4)) return SK_ERR_BAD_ALIGNMENT;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
   LaunchConfig lc(blocks, matrices, 256, 0, false, 1, static_cast<cudaStream_t>(stream));
@@ -537,6 +542,7 @@ int sk_route_tokens(const void* logits, int logits_type, int64_t ld, int64_t T, 
   if (!is_float_type(logits_type)) return SK_ERR_BAD_ARGUMENT;
   if (int rc = check_route(T, E, k); rc != SK_OK) return rc;
   if (ld < E) return SK_ERR_BAD_SHAPE;
+  if (!aligned(logits, logits_type == SK_FLOAT_F32 ? 4 : 2) || !aligned4({ids, weights, rows, offsets})) return SK_ERR_BAD_ALIGNMENT;
   RouteParams p = {};
   p.logits = logits;
   p.ld = ld;
@@ -553,6 +559,7 @@ int sk_group_by_expert(const int32_t* ids, int64_t T, int64_t k, int64_t E, int3
   if (!ids || !rows || !offsets) return SK_ERR_NULL_POINTER;
   if (int rc = check_route(T, E, 1); rc != SK_OK) return rc;
   if (k < 1 || k > 1024 || T * k > kIntMax) return SK_ERR_BAD_SHAPE;
+  if (!aligned4({ids, rows, offsets})) return SK_ERR_BAD_ALIGNMENT;
   RouteParams p = {};
   p.ids = const_cast<int32_t*>(ids);               // (only read)
   p.rows = rows;
@@ -576,7 +583,7 @@ int sk_fp8_experts(int64_t T, int64_t k, const void* x, int x_type, int64_t ld_x
   if (gate_up->experts != 2 * E || gate_up->N != inter || gate_up->K != hidden || ld_x < hidden) return SK_ERR_BAD_SHAPE;
   if (k < 1 || k > 1024 || T * k > kIntMax - 4096) return SK_ERR_BAD_SHAPE;
   if (!is_float_type(x_type) || workspace_bytes < sk_fp8_experts_workspace_bytes(T, k, hidden, inter, scale_type)) return SK_ERR_BAD_ARGUMENT;
-  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(workspace, 256)) return SK_ERR_BAD_ALIGNMENT;
+  if (!aligned(x, x_type == SK_FLOAT_F32 ? 4 : 2) || !aligned(workspace, 256) || !aligned4({rows, weights, offsets})) return SK_ERR_BAD_ALIGNMENT;
   if (T == 0) return SK_OK;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t R = T * k, ld_y = round_up(hidden, 16);
