@@ -117,9 +117,18 @@ def _padded_codes(w, scale_dtype):
 
 
 class _KeepsTypes(nn.Module):
-    """Codes and scales are moved as they are: `.half()` and `.to(dtype)` are for what a model computes in, not for them."""
+    """Codes and scales are moved as they are: `.half()`, `.to(dtype)` and `.type(dtype)` are for what a model computes in, not for them, and
+    a memory format is for its images."""
 
     _as_they_are = ()
+
+    @staticmethod
+    def _moved(fn, t):
+        flat = t.reshape(-1).view(torch.uint8)          # (one row of bytes: casts of floats and memory formats pass it by)
+        moved = fn(flat)
+        if moved.dtype != flat.dtype:                   # (`.type(dtype)` casts whatever it meets)
+            moved = flat.to(moved.device)
+        return moved.view(t.dtype).view(t.shape)
 
     def _apply(self, fn, recurse=True):
         held = {name: self._buffers[name] for name in self._as_they_are}
@@ -127,7 +136,7 @@ class _KeepsTypes(nn.Module):
             self._buffers[name] = None
         try:
             super()._apply(fn, recurse)
-            moved = {name: fn(t.view(torch.uint8 if t.element_size() == 1 else torch.int32)).view(t.dtype) for name, t in held.items()}
+            moved = {name: self._moved(fn, t) for name, t in held.items()}
         except BaseException:
             self._buffers.update(held)
             raise
