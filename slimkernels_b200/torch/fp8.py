@@ -131,7 +131,7 @@ class _KeepsTypes(nn.Module):
         return moved.view(t.dtype).view(t.shape)
 
     def _apply(self, fn, recurse=True):
-        held = {name: self._buffers[name] for name in self._as_they_are}
+        held = {name: t for name in self._as_they_are if (t := self._buffers.get(name)) is not None}
         for name in held:
             self._buffers[name] = None
         try:

@@ -47,3 +47,15 @@ def test_shared_memory_is_shared():
     m = _modules()[0]
     m.share_memory()
     assert m.w_q.untyped_storage().is_shared() and m.w_scale.untyped_storage().is_shared()
+
+
+def test_a_weight_that_is_no_buffer_any_more_may_be_moved():
+    m = _modules()[0]
+    codes = m.w_q.clone()
+    m.w_q = nn.Parameter(codes, requires_grad=False)
+    assert m.to("cpu").w_q.dtype == codes.dtype and m.to("meta").w_q.is_meta
+    m = _modules()[0]
+    m.register_buffer("bias", None)
+    del m.w_scale
+    m.w_scale = torch.ones(1, 2)                            # (a plain attribute from now on)
+    assert m.half().w_q.dtype == codes.dtype
