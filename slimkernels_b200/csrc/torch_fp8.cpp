@@ -1,5 +1,6 @@
 // The FP8 ops of namespace `slimkernels` (slimkernels_b200/torch/fp8.py): tensors into the C ABI of include/sk_fp8.h.  No kernels
 // live here.  Inference only, like the W2A8 ops: nothing is recorded for a backward pass.
+#include <ATen/Context.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -21,8 +22,11 @@ void check(int rc, const char* what) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
-// at::empty on like's device without a turn through the dispatcher (0.4 us each; a router call makes four).
+// at::empty on like's device without a turn through the dispatcher (0.4 us each; a router call makes four), so dispatch modes do not see it.
+// torch's deterministic mode, which fills new tensors, has its turn.
 at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
+  const at::Context& context = at::globalContext();
+  if (C10_UNLIKELY(context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory())) return at::empty(size, like.options().dtype(type));
   return at::Tensor(at::detail::empty_cuda(size, type, like.device(), c10::nullopt));
 }
 
