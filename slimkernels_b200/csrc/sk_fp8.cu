@@ -154,6 +154,30 @@ int with_type(int t, F&& fn) {
 }
 
 // ---------------------------------------------------------------- products
+constexpr int kSmShared = 233472, kCtaShared = 232448;      // shared memory of an SM (1 KiB per CTA goes to the system) and of a CTA
+constexpr int shared_for(int ctas) { return ctas == 1 ? kCtaShared : kSmShared / ctas - 1024; }      // what a CTA may have with so many to an SM
+
+// How many clusters of 2, 4 or 8 CTAs, one or two CTAs to an SM, run at once.  A cluster lies within one GPC, so fewer fit than there is room for
+// single CTAs: on B200's 148 SMs 33 of four and 15 of eight, with two CTAs to an SM 71 and 33.  Asked for a kernel of its own, which is never launched:
+// of a kernel that takes tensor memory the occupancy calculator only counts one CTA to an SM, though two run (72 clusters of four are slower than 71 by a third).
+__global__ void cluster_room_kernel() {}
+int clusters_at_once(const DeviceInfo& dev, int size, int per_sm) {
+  static std::atomic<int> known[64][2][4];
+  std::atomic<int>& slot = known[dev.index][per_sm - 1][size == 2 ? 1 : size == 4 ? 2 : 3];
+  int n = slot.load();
+  if (n == 0) {
+    static std::atomic<uint64_t> done;
+    LaunchConfig lc(size, 1, 256, shared_for(per_sm), false, size, nullptr);
+    if (allow_shared(cluster_room_kernel, kCtaShared, dev, done) != SK_OK ||
+        cudaOccupancyMaxActiveClusters(&n, cluster_room_kernel, &lc.cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    slot.store(n);
+  }
+  return n;
+}
+
 struct Choice {
   int kernel;                           // sk_fp8_kernel
   int row_tile, feature_tile, split;
@@ -175,10 +199,19 @@ struct Choice {
 //     tile 16  21.9 / 27.0 / 33.4 / 47.8     many  28.7 / 29.8 / 31.0 / 31.4
 //   With the SiLU epilogue, whose time goes with the tile's rows, tiles of 16 are the fastest up to 32 rows per expert (67 us a block, tiles of 32 87, many 80).
 // A tile's K range is split while that leaves an SM for every CTA and a CTA eight K blocks or so: 64 x 4096 x 4096 12.9 us in one, 10.9 in four; splitting
-// where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two; 256 x 2048 x 4096, 8-bit scales, 11.1 and 11.7).  Two CTAs to an SM
-// are better only where K is long -- 32-bit scales: 100 x 1000 x 8192 13.2 in two, 9.6 in four; 300 x 512 x 16384 33.5 in one, 22.4 in two; 8-bit scales: 300 x 512
-// x 16384 19.6 in two, 14.1 in four; 16 x 8192 x 16384 26.7 and 24.8; but 100 x 1000 x 8192 9.1 in four and in eight.
-Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, int sms) {
+// where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two; 256 x 2048 x 4096, 8-bit scales, 11.1 and 11.7).
+// Beyond that, to two CTAs an SM, it is split where all clusters run at once (16 x 9216 x 16384, 72 tiles: four 35.6, two 28.5; 71 tiles 28.3) and K is long (us, a
+// quarter GB of weights in turn).  From one to two:
+//   32-bit scales, one row tile:   80 feature tiles  K 4096 12.7 / 12.5  6144 17.0 / 14.7    112  4096 13.6 / 14.3  6144 18.7 / 17.9
+//                                  144               4096 15.2 / 17.1  6144 21.4 / 22.1  8192 27.6 / 27.0
+//     where weights are read again by other row tiles:   40 x 2  4096 12.1 / 10.2    72 x 2  4096 12.6 / 12.7  6144 16.8 / 15.0    18 x 8  4096 12.1 / 10.6
+//   8-bit scales:   40 x 2  8192 18.1 / 17.5    56 x 2  8192 18.2 / 18.5    72 x 2  18.5 / 21.2    36 x 4  18.3 / 17.8    18 x 8  18.3 / 17.2
+//                   one row tile   80  19.0 / 18.0    96  19.5 / 20.8    112  22.5 / 22.7    144  27.2 / 27.5
+//   so the more feature tiles, that is the nearer to the stream of weights, the longer K has to be, and with 8-bit scales there are too many at two fifths of the SMs.
+//   From two to four, 32-bit scales, K 8192:   56  15.2 / 14.2   70  16.4 / 16.8   28 x 2  14.0 / 11.3;   8-bit scales, K 16384:   56  23.8 / 22.0   70  28.3 / 27.0
+//   14 x 4  20.1 / 16.5, but K 8192   56  14.2 / 14.2.
+Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bool silu, bool e8m0, const DeviceInfo& dev) {
+  const int sms = dev.sms;
   Choice c;
   const int64_t rows = ceil_div(M, experts);       // of a group, on average
   const int64_t blocks = ceil_div(N, 128), kb = ceil_div(K, 128);
@@ -206,7 +239,8 @@ Choice choose(int64_t M, int64_t N, int64_t K, int64_t experts, bool grouped, bo
   c.split = 1;
   if (!grouped && few) {
     while (c.split < 8 && tiles * c.split * 2 <= sms && kb >= c.split * 8) c.split *= 2;
-    while (c.split < 8 && tiles * c.split * 2 <= 2 * sms && kb >= c.split * (e8m0 ? 64 : 32)) c.split *= 2;
+    const bool streams = e8m0 ? blocks * 5 > sms * 2 : kb * 5 < blocks * 2;
+    while (c.split < 8 && tiles <= clusters_at_once(dev, c.split * 2, 2) && kb >= c.split * (e8m0 ? 64 : 32) && !(c.split == 1 && streams)) c.split *= 2;
     if (const int64_t forced = g_options[SK_FP8_OPT_SPLIT_K].load()) c.split = forced <= kb ? static_cast<int>(forced) : 1;
   }
   c.ctas = tiles * c.split;
@@ -236,19 +270,21 @@ int launch_wide(const CUtensorMap& mw, const CUtensorMap& mx, const Fp8Params& p
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
 }
 
-// The ring: 3 to 12 stages, for two CTAs per SM where there are more CTAs than SMs and two fit, else for one.
+// The ring: 3 to 12 stages, for two CTAs per SM where there are more CTAs than SMs and two fit, else for one.  The clusters of a split
+// count as they fit: 16 of eight CTAs with an SM each ran one after 15 others (1 x 2048 x 4096 10.5 us, 5.8 with two CTAs to an SM), 36 of four after 33 (1 x 4608
+// x 4096 13.3 and 7.7).
 template <int TOK, bool SILU>
 int launch_scaled_narrow(const CUtensorMap& mw, const CUtensorMap& mx, Fp8Params p, int64_t tiles, const DeviceInfo& dev, cudaStream_t stream) {
   using T = Fp8ScaledNarrowTraits<TOK, SILU>;
   auto kern = fp8_scaled_narrow_kernel<TOK, SILU>;
-  constexpr int kSm = 233472, kCta = 232448;        // shared memory of an SM (1 KiB per CTA goes to the system) and of a CTA
   const int fixed = T::fixed_bytes(p.split, p.experts);
-  int ctas = tiles * p.split > dev.sms ? 2 : 1;
-  if ((kSm / ctas - 1024 - fixed) / T::kStageBytes < 3) ctas = 1;
-  p.stages = std::min(T::kMaxStages, ((ctas == 1 ? kCta : kSm / 2 - 1024) - fixed) / T::kStageBytes);
-  static_assert((kCta - T::fixed_bytes(SILU ? 1 : 8, 1)) / T::kStageBytes >= 3 && (kCta - T::fixed_bytes(1, kFp8MaxExperts)) / T::kStageBytes >= 3, "room for a ring");
+  int ctas = (p.split > 1 ? tiles > clusters_at_once(dev, p.split, 1) : tiles > dev.sms) ? 2 : 1;
+  if ((shared_for(ctas) - fixed) / T::kStageBytes < 3) ctas = 1;
+  p.stages = std::min(T::kMaxStages, (shared_for(ctas) - fixed) / T::kStageBytes);
+  static_assert((kCtaShared - T::fixed_bytes(SILU ? 1 : 8, 1)) / T::kStageBytes >= 3 && (kCtaShared - T::fixed_bytes(1, kFp8MaxExperts)) / T::kStageBytes >= 3,
+                "room for a ring");
   static std::atomic<uint64_t> done;
-  if (int rc = allow_shared(kern, kCta, dev, done); rc != SK_OK) return rc;
+  if (int rc = allow_shared(kern, kCtaShared, dev, done); rc != SK_OK) return rc;
   const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, static_cast<int64_t>(dev.sms) * ctas);
   LaunchConfig lc(grid, 1, T::kThreads, fixed + p.stages * T::kStageBytes, true, p.split, stream);
   return cuda_status(cudaLaunchKernelEx(&lc.cfg, kern, mw, mx, p));
@@ -288,7 +324,7 @@ int product(int64_t M, const sk_fp8_rows* x, const sk_fp8_weight* w, int scale_t
   const int64_t N = w->N, K = w->K;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
-  const Choice c = choose(M, N, K, experts, offsets != nullptr, silu, scale_type == SK_SCALE_E8M0, dev.sms);
+  const Choice c = choose(M, N, K, experts, offsets != nullptr, silu, scale_type == SK_SCALE_E8M0, dev);
   Fp8Params p = {};
   p.x_scale = x->scale;
   p.xs_row = x->scale_row;
@@ -633,7 +669,7 @@ int sk_fp8_query_launch(int64_t M, int64_t N, int64_t K, int64_t experts, int sc
   if (!is_scale_type(scale_type)) return SK_ERR_BAD_ARGUMENT;
   DeviceInfo dev;
   if (int rc = device_info(&dev); rc != SK_OK) return rc;
-  const Choice c = choose(M, N, K, experts, experts > 1, false, scale_type == SK_SCALE_E8M0, dev.sms);
+  const Choice c = choose(M, N, K, experts, experts > 1, false, scale_type == SK_SCALE_E8M0, dev);
   if (kernel) *kernel = c.kernel;
   if (row_tile) *row_tile = c.row_tile;
   if (feature_tile) *feature_tile = c.feature_tile;
