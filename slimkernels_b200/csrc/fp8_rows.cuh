@@ -73,8 +73,8 @@ template <int TYPE, bool E8M0, bool VECTOR>
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(const void* x, long long ld_x, long long M, int K, uint8_t* q, long long ld_q, void* scale, long long s_row,
                     long long s_blk, const int* rows, int choices, int places) {
-  // The next kernel may start only when every CTA of this one has passed the wait: what it then reads early (weights) was complete
-  // before this kernel's inputs were.
+  // The next kernel may start only when every CTA of this one has passed the wait: what it then reads early (weights, offsets) was
+  // complete before this kernel's inputs were.  So the trigger has to stay behind the wait (the products' stand in front of theirs).
   grid_dep_wait();
   grid_dep_launch_dependents();
   // A CTA takes 16 neighbouring blocks (blockIdx.y) of every gridDim.x-th row, two rows a turn; a row's destinations come with its values, one

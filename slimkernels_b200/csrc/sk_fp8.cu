@@ -103,9 +103,11 @@ bool is_float_type(int t) { return t >= SK_FLOAT_F16 && t <= SK_FLOAT_F32; }
 bool is_out_type(int t) { return t == SK_OUT_F16 || t == SK_OUT_BF16; }
 int64_t scale_bytes(int scale_type) { return scale_type == SK_SCALE_E8M0 ? 1 : 4; }
 
-// dependent: programmatic dependent launch.  Every kernel here but the weight preparation waits (griddepcontrol.wait) before it reads or
-// writes global memory, so its set-up may run under the tail of whatever is in front of it; that saves 1 to 2 us a launch between
-// this library's kernels, which let their followers start early.  (A follower may hold tensor memory while it waits.  It cannot take any that the
+// dependent: programmatic dependent launch.  Every kernel here but the weight preparation waits (griddepcontrol.wait) before it reads what a
+// kernel still in flight may write, and before it writes anything, so its set-up may run under the tail of whatever is in front of it; that saves 1 to 2
+// us a launch between this library's kernels, which let their followers start early.  Products of a call with the quantiser in front of them
+// (early_weights) read weights and offsets before their wait.  That is sound only because fp8_quantize_kernel lets its followers start AFTER its own
+// wait: see product().  (A follower may hold tensor memory while it waits.  It cannot take any that the
 // kernel in front still needs: every kernel here takes at most half of an SM's columns with half of its shared memory, or all with most of it.)
 struct LaunchConfig {
   cudaLaunchConfig_t cfg = {};
