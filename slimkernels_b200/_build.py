@@ -52,6 +52,9 @@ def build_cuda_lib(force: bool = False, verbose: bool = False, ptxas_info: bool 
               [os.path.join(_ROOT, "include", f) for f in ("sk_w2a8.h", "sk_fp8.h")]
     units = {"sk_w2a8": [h for h in headers if not os.path.basename(h).startswith(("fp8_", "sk_fp8"))],
              "sk_fp8": [h for h in headers if not os.path.basename(h).startswith("w2a8_")]}
+    sources = [os.path.join(_CSRC, unit + ".cu") for unit in units]
+    if not force and not _newer(CUDA_LIB, sources + headers):      # (a library may come without its objects, and without nvcc)
+        return CUDA_LIB
     os.makedirs(LIB_DIR, exist_ok=True)
     objects, jobs = [], []
     for unit, deps in units.items():
