@@ -5,7 +5,7 @@
 // that happens to it is a copy, four MMAs and a commit: what the kernel for 32-bit scales does per K block in its epilogue -- 700
 // cycles for one CTA, which held a projection of 4096 features and 16 rows to 44 GB/s per CTA -- is gone, and the stream is as fast as the ring
 // is deep: 16 x 18944 x K, a tile per SM, takes 3.4 us and then 6.2 TB/s.  (One SM draws 80 GB/s at most.)  The ring takes what shared
-// memory there is: where a call has no more CTAs than SMs, all of it for one CTA, else half.
+// memory there is: where all CTAs (or all clusters of a split) run at once with an SM each, all of it for one CTA, else half.
 //
 // A tile's K range can be split over a cluster: every CTA pushes its sums into the CTA that owns the row (remote stores), one cluster
 // barrier, then the owner adds them in rank order, so the result does not depend on timing.

@@ -197,10 +197,11 @@ struct Choice {
 //     tile 16  21.7 / 26.1 / 26.8 / 31.4 / 41.9     tile 32  22.5 / 25.8 / 25.9 / 29.2 / 34.4
 //     many     27.1 / 26.3 / 26.5 / 27.1 / 27.7 / 49.9 / 135.6     pair  30.1 / 31.2 / 32.1 / 33.1 / 34.3 / 48.7 / 126.4
 //   (64 experts x 2048 x 2048 at 16 and 32: tile 32  47.9, 50.3, many  50.2, 51.4).  A pair's tiles of 256 rows are emptier at a group's end, which costs
-//   more than its faster MMAs give up to about 512 rows (expert layers of 512 rows each: many 195, pair 201).  With 32-bit scales, 2 / 16 / 32 / 64:
+//   more than its faster MMAs give up to about 512 rows (16 experts' layers of 2048 x 1024, 512 rows each: many 129, pair 145; 1024 rows 238 and 235).
+//   With 32-bit scales, 2 / 16 / 32 / 64:
 //     tile 16  21.9 / 27.0 / 33.4 / 47.8     many  28.7 / 29.8 / 31.0 / 31.4
 //   With the SiLU epilogue, whose time goes with the tile's rows, tiles of 16 are the fastest up to 32 rows per expert (67 us a block, tiles of 32 87, many 80).
-// A tile's K range is split while that leaves an SM for every CTA and a CTA eight K blocks or so: 64 x 4096 x 4096 12.9 us in one, 10.9 in four; splitting
+// A tile's K range is split while that makes no more CTAs than SMs and leaves a CTA eight K blocks or so: 64 x 4096 x 4096 12.9 us in one, 10.9 in four; splitting
 // where the tiles fill the SMs already loses (16 x 22016 x 4096 18.8 in one, 25.2 in two; 256 x 2048 x 4096, 8-bit scales, 11.1 and 11.7).
 // Beyond that, to two CTAs an SM, it is split where all clusters run at once (16 x 9216 x 16384, 72 tiles: four 35.6, two 28.5; 71 tiles 28.3) and K is long (us, a
 // quarter GB of weights in turn).  From one to two:

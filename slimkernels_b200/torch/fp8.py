@@ -146,7 +146,8 @@ class _KeepsTypes(nn.Module):
 
 class FP8Linear(_KeepsTypes):
     """y = x W^T (+ bias) with an 8-bit weight and activations quantised on the way.  w_q float8_e4m3fn [out_features, in_features
-    padded to a multiple of 16], w_scale [ceil(out / 128), ceil(in / 128)]."""
+    padded to a multiple of 16], w_scale [ceil(out / 128), ceil(in / 128)].  The product is rounded to out_dtype, then the sum with the bias, as in
+    the 2-bit layers."""
 
     _as_they_are = ("w_q", "w_scale")
 
