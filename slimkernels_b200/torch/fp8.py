@@ -111,6 +111,8 @@ def fp8_device_status(device=None) -> int:
 
 def _padded_codes(w, scale_dtype):
     """Codes whose rows are padded to a multiple of 16, as a whole tensor (what a module keeps: it survives .to() and a state dict)."""
+    if w.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        w = w.to(torch.float32)
     codes, scale = prepare_weight_fp8(w, scale_dtype)
     full = codes.as_strided((*codes.shape[:-1], codes.stride(-2)), codes.stride()) if codes.stride(-2) != codes.shape[-1] else codes
     return full, scale

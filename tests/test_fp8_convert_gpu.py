@@ -52,3 +52,22 @@ def test_one_projection_in_8_bits(name, dtype):
             assert torch.equal(got, want) and bool(torch.isfinite(got).all())
             assert isinstance(getattr(model[key], name), sk.FP8Linear)
     assert type(model["skipped"].down_proj) is (sk.FP8Linear if name == "down_proj" else nn.Linear)
+
+
+class _Experts(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.gate_up_proj, self.down_proj, self.act_fn = nn.Parameter(torch.randn(3, 96, 64)), nn.Parameter(torch.randn(3, 64, 48)), nn.SiLU()
+
+
+def test_weights_of_other_float_types_are_taken_as_by_the_2_bit_layers():
+    torch.manual_seed(6)
+    model = nn.ModuleDict({"experts": _Experts(), "head": nn.Linear(128, 40), "proj": nn.Linear(128, 40)}).cuda().double()
+    plain = copy.deepcopy(model).float()
+    assert sk.quantize_linears(model, fp8=("head",), experts=True) == {"linear": 1, "mlp": 0, "kept": [], "fp8": 1, "experts": 1}
+    same = sk.FP8Linear.from_float(plain["head"].weight, plain["head"].bias)
+    for n in ("w_q", "w_scale", "bias"):
+        a, b = getattr(model["head"], n), getattr(same, n)
+        assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    same = sk.FP8Experts.from_float(plain["experts"].gate_up_proj, plain["experts"].down_proj)
+    assert all(torch.equal(getattr(model["experts"], n).view(torch.uint8), getattr(same, n).view(torch.uint8)) for n in same._as_they_are)
