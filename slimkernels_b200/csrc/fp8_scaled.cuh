@@ -201,6 +201,11 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             if (++stage == S) { stage = 0; phase ^= 1; }
           }
         }
+        // A pair's second CTA leaves only when the first one's arrivals on its barriers have all landed: the sums' barrier, which the epilogue waits
+        // for, says nothing of the others'.
+        if constexpr (CTAS == 2)
+          for (int i = 0; i < S && ok; ++i)
+            ok = wait_bounded_relaxed(bar_done + 8 * ((stage + i) % S), stage + i < S ? phase : phase ^ 1, ctx, kStProducerEmpty, 40);
         if (!ok) {
           // Gave up: no copy may be in flight into this CTA's memory when it exits.  The first CTA watches the barriers that count
           // them, and the second, which cannot, waits far longer than a copy takes; it leaves after the first in any case.
@@ -300,6 +305,12 @@ fp8_scaled_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           if (++slot == T::kSlots) { slot = 0; phase ^= 1; }
         }
       }
+      if constexpr (CTAS == 2)                        // (see the producer)
+        for (int i = 0; i < T::kSlots && ok; ++i) {
+          ok = wait_bounded_relaxed(bar_scales_free + 8 * slot, phase, ctx, kStProducerEmpty, 40);
+          ok = __all_sync(0xffffffffu, ok);
+          if (++slot == T::kSlots) { slot = 0; phase ^= 1; }
+        }
       __syncwarp();
     }
   } else {
